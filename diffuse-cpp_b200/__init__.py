@@ -438,3 +438,10 @@ class Context:
 from . import dp  # noqa: E402  (data-parallel plumbing over independent sequences)
 from . import serve  # noqa: E402  (request server over a pool of contexts)
 from . import tp  # noqa: E402  (tensor-parallel shard plan and its numpy execution)
+
+
+def __getattr__(name):
+    if name == "ops":  # operators on torch device tensors: torch is imported on first use
+        import importlib
+        return importlib.import_module(".ops", __name__)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -29,13 +29,14 @@
 #include "../../../include/diffuse_b200.h"
 #include "attention.cuh"
 #include "gemm_dq.cuh"
+#include "host_util.h"
 #include "ops.cuh"
 
 using namespace dfb;
 
 // ───────────────────────── errors ─────────────────────────
 static thread_local std::string g_err;
-static int set_err(int code, const char *fmt, ...) {
+int dfb::set_err(int code, const char *fmt, ...) {
     char buf[1024];
     va_list ap;
     va_start(ap, fmt);
@@ -44,18 +45,6 @@ static int set_err(int code, const char *fmt, ...) {
     g_err = buf;
     return code;
 }
-#define CK(call)                                                                                   \
-    do {                                                                                           \
-        cudaError_t e_ = (call);                                                                   \
-        if (e_ != cudaSuccess)                                                                     \
-            return set_err(e_ == cudaErrorMemoryAllocation ? DFB_ERR_NOMEM : DFB_ERR_CUDA,         \
-                           "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
-    } while (0)
-#define RET(x)                 \
-    do {                       \
-        int r_ = (x);          \
-        if (r_ != DFB_OK) return r_; \
-    } while (0)
 
 extern "C" const char *dfb_last_error(void) { return g_err.c_str(); }
 
@@ -907,31 +896,12 @@ static void prof_collect(dfb_ctx *c, int M) {
     c->prof_pending.clear();
 }
 
-// Programmatic dependent launch: a kernel launched this way may start while the
-// previous kernel of the stream is finishing; every such kernel executes
-// griddepcontrol.wait before it touches memory the previous kernels write.
-// DIFFUSE_PDL=0 turns it off (plain stream order).
-static bool pdl_enabled() {
+bool dfb::pdl_enabled() {
     static const bool on = [] {
         const char *e = getenv("DIFFUSE_PDL");
         return !(e && e[0] == '0');
     }();
     return on;
-}
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_k(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl,
-                            Args... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = (pdl && pdl_enabled()) ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
 // CTA pairs of a GEMM instantiation that fit on the device at once (one CTA per SM).

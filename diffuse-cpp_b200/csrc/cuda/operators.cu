@@ -1,0 +1,202 @@
+// Entry points of the operators on device tensors (include/diffuse_b200.h): argument checks, the
+// choice of a kernel variant, launches.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "host_util.h"
+#include "kv_append.cuh"
+#include "kv_attention.cuh"
+#include "logprobs.cuh"
+
+using namespace dfb;
+
+namespace {
+
+enum { T_F32 = 0, T_F16 = 1, T_BF16 = 30 };
+int type_size(int t) { return t == T_F32 ? 4 : 2; }
+
+// The calling thread's device while a call works on another one.
+class DeviceGuard {
+  public:
+    // the device that holds p; false with an error recorded when p is no device memory
+    int enter(const void *p, const char *what) {
+        cudaPointerAttributes at{};
+        const cudaError_t e = cudaPointerGetAttributes(&at, p);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return set_err(e == cudaErrorInvalidValue ? DFB_ERR_ARG : DFB_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+        }
+        if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+            return set_err(DFB_ERR_ARG, "%s is not device memory", what);
+        dev_ = at.device;
+        CK(cudaGetDevice(&old_));
+        if (old_ != dev_) CK(cudaSetDevice(dev_));
+        return DFB_OK;
+    }
+    ~DeviceGuard() {
+        if (old_ >= 0 && old_ != dev_) cudaSetDevice(old_);
+    }
+    int device() const { return dev_; }
+
+  private:
+    int dev_ = -1, old_ = -1;
+};
+
+// Compute capability and SM count, looked up once per device.
+int device_props(int dev, int *n_sm) {
+    static int sms[64] = {0};
+    if (dev < 0 || dev >= 64) return set_err(DFB_ERR_UNSUPPORTED, "device %d", dev);
+    if (!sms[dev]) {
+        int major = 0, n = 0;
+        CK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+        CK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        if (major != 10) return set_err(DFB_ERR_UNSUPPORTED, "device %d is sm_%d; this build targets sm_100a", dev, 10 * major);
+        sms[dev] = n;
+    }
+    *n_sm = sms[dev];
+    return DFB_OK;
+}
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_cache(const dfb_kv_cache *c) {
+    if (!c) return set_err(DFB_ERR_ARG, "null cache");
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->pages) return set_err(DFB_ERR_ARG, "null pointer in the cache");
+    if (c->head_dim != 64 && c->head_dim != 128) return set_err(DFB_ERR_UNSUPPORTED, "head_dim %d not supported (64/128)", c->head_dim);
+    if (c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
+        return set_err(DFB_ERR_UNSUPPORTED, "page of %d positions not supported (16/32/64/128)", c->page);
+    if (c->n_pages <= 0 || c->n_kv <= 0 || c->n_seq <= 0 || c->max_pages <= 0)
+        return set_err(DFB_ERR_ARG, "cache of %d pages, %d KV heads, %d sequences of %d pages", c->n_pages, c->n_kv, c->n_seq, c->max_pages);
+    if (c->n_seq > 65535 || c->n_kv > 8192) return set_err(DFB_ERR_UNSUPPORTED, "%d sequences / %d KV heads", c->n_seq, c->n_kv);
+    if ((int64_t)c->max_pages * c->page > INT32_MAX) return set_err(DFB_ERR_UNSUPPORTED, "page table of %d pages", c->max_pages);
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return set_err(DFB_ERR_ARG, "cache codes not 16-byte aligned");
+    return DFB_OK;
+}
+
+// Strides of a [rows][heads][head_dim] tensor of caller memory: not negative (a row is the last one plus).
+int check_rows(const char *what, const void *p, int type, int64_t tok, int64_t head) {
+    if (!p) return set_err(DFB_ERR_ARG, "null %s", what);
+    if (!aligned(p, type_size(type))) return set_err(DFB_ERR_ARG, "%s not aligned to its type", what);
+    if (tok < 0 || head < 0) return set_err(DFB_ERR_ARG, "%s has a negative stride", what);
+    return DFB_OK;
+}
+// Whether eight consecutive values of every row can be moved as 16-byte pieces.
+bool vec_ok(const void *p, int type, int64_t tok, int64_t head) {
+    const int64_t n = 16 / type_size(type);
+    return aligned(p, 16) && tok % n == 0 && head % n == 0;
+}
+
+template <typename T, int HD>
+int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, bool vec, dim3 grid, int32_t *status, cudaStream_t st) {
+    const int items = c.page * (HD / 16);
+    if (items <= kAppendThreads) kv_append_kernel<T, HD, 1><<<grid, kAppendThreads, 0, st>>>(c, r, vec, status);
+    else if (items <= 2 * kAppendThreads) kv_append_kernel<T, HD, 2><<<grid, kAppendThreads, 0, st>>>(c, r, vec, status);
+    else kv_append_kernel<T, HD, 4><<<grid, kAppendThreads, 0, st>>>(c, r, vec, status);
+    CK(cudaGetLastError());
+    return DFB_OK;
+}
+
+template <typename T, int HD>
+int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, int32_t *status, cudaStream_t st) {
+    kv_attn_simple<T, HD><<<dim3((a.max_rows + 3) / 4, a.n_q, c.n_seq), 128, 0, st>>>(c, a, status);
+    CK(cudaGetLastError());
+    return DFB_OK;
+}
+
+int check_attn(const dfb_kv_cache *c, const dfb_kv_attn *a) {
+    RET(check_cache(c));
+    if (!a) return set_err(DFB_ERR_ARG, "null arguments");
+    if (a->type != T_F16 && a->type != T_BF16) return set_err(DFB_ERR_UNSUPPORTED, "query type %d not supported (F16 / BF16)", a->type);
+    if (a->n_q <= 0 || a->n_q % c->n_kv) return set_err(DFB_ERR_ARG, "%d query heads over %d KV heads", a->n_q, c->n_kv);
+    if (a->n_q > 65535) return set_err(DFB_ERR_UNSUPPORTED, "%d query heads", a->n_q);
+    if (a->n_rows < 0 || a->max_rows < 0 || a->max_keys < 0) return set_err(DFB_ERR_ARG, "negative size");
+    if (!std::isfinite(a->scale)) return set_err(DFB_ERR_ARG, "scale must be finite");
+    return DFB_OK;
+}
+
+}  // namespace
+
+extern "C" int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_t *status, void *stream) {
+    RET(check_cache(c));
+    if (!r) return set_err(DFB_ERR_ARG, "null arguments");
+    if (r->type != T_F32 && r->type != T_F16 && r->type != T_BF16) return set_err(DFB_ERR_UNSUPPORTED, "row type %d not supported", r->type);
+    if (r->n_rows < 0 || r->max_rows < 0) return set_err(DFB_ERR_ARG, "negative size");
+    if (r->n_rows == 0 || r->max_rows == 0) return DFB_OK;
+    RET(check_rows("k", r->k, r->type, r->k_tok, r->k_head));
+    RET(check_rows("v", r->v, r->type, r->v_tok, r->v_head));
+    if (!r->row_off || !r->len) return set_err(DFB_ERR_ARG, "null row offsets or lengths");
+    if (r->rope && (r->n_rope <= 0 || !aligned(r->rope, 16))) return set_err(DFB_ERR_ARG, "rotation table empty or not 16-byte aligned");
+    if (r->q) {
+        if (r->n_q <= 0 || r->n_q > 8192) return set_err(DFB_ERR_ARG, "%d query heads", r->n_q);
+        RET(check_rows("q", r->q, r->type, r->q_tok, r->q_head));
+        RET(check_rows("q_out", r->q_out, r->type, r->q_out_tok, r->q_out_head));
+    }
+    DeviceGuard g;
+    RET(g.enter(c->k, "the cache"));
+    int n_sm = 0;
+    RET(device_props(g.device(), &n_sm));
+    bool vec = vec_ok(r->k, r->type, r->k_tok, r->k_head) && vec_ok(r->v, r->type, r->v_tok, r->v_head);
+    if (r->q) vec = vec && vec_ok(r->q, r->type, r->q_tok, r->q_head) && vec_ok(r->q_out, r->type, r->q_out_tok, r->q_out_head);
+    // pages a sequence's rows can touch: consecutive positions n / page + 2 at most, given positions any of them
+    const int64_t most = r->pos ? c->max_pages : std::min<int64_t>(c->max_pages, ((int64_t)r->max_rows + c->page - 2) / c->page + 1);
+    const dim3 grid((unsigned)most, 2 * c->n_kv + (r->q ? r->n_q : 0), c->n_seq);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        return c->head_dim == 64 ? append_t<T, 64>(*c, *r, vec, grid, status, st) : append_t<T, 128>(*c, *r, vec, grid, status, st);
+    };
+    return r->type == T_F32 ? go(float()) : r->type == T_F16 ? go(__half()) : go(__nv_bfloat16());
+}
+
+extern "C" int dfb_kv_attention_workspace(const dfb_kv_cache *c, const dfb_kv_attn *a, size_t *bytes) {
+    if (!bytes) return set_err(DFB_ERR_ARG, "null pointer");
+    *bytes = 0;
+    return DFB_OK;
+}
+
+extern "C" int dfb_kv_attention(const dfb_kv_cache *c, const dfb_kv_attn *a, void *workspace, size_t ws_bytes, int32_t *status,
+                                void *stream) {
+    RET(check_attn(c, a));
+    if (a->n_rows == 0 || a->max_rows == 0) return DFB_OK;
+    RET(check_rows("q", a->q, a->type, a->q_tok, a->q_head));
+    RET(check_rows("out", a->out, a->type, a->out_tok, a->out_head));
+    if (!a->row_off || !a->len) return set_err(DFB_ERR_ARG, "null row offsets or lengths");
+    DeviceGuard g;
+    RET(g.enter(c->k, "the cache"));
+    int n_sm = 0;
+    RET(device_props(g.device(), &n_sm));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->type == T_F16) return c->head_dim == 64 ? attn_t<__half, 64>(*c, *a, status, st) : attn_t<__half, 128>(*c, *a, status, st);
+    return c->head_dim == 64 ? attn_t<__nv_bfloat16, 64>(*c, *a, status, st) : attn_t<__nv_bfloat16, 128>(*c, *a, status, st);
+}
+
+extern "C" int dfb_token_logprobs(const dfb_logprob_args *a, int32_t *status, void *stream) {
+    if (!a) return set_err(DFB_ERR_ARG, "null arguments");
+    if (a->type != T_F32 && a->type != T_F16 && a->type != T_BF16) return set_err(DFB_ERR_UNSUPPORTED, "logits type %d not supported", a->type);
+    if (a->n_rows < 0 || a->n_logits < 0) return set_err(DFB_ERR_ARG, "negative size");
+    if (a->n_vocab <= 0) return set_err(DFB_ERR_ARG, "vocabulary of %d", a->n_vocab);
+    if (a->ld < a->n_vocab && a->n_logits > 1) return set_err(DFB_ERR_ARG, "row stride %lld < %d", (long long)a->ld, a->n_vocab);
+    if (a->top_k < 0 || a->top_k > 32 || a->top_k > a->n_vocab) return set_err(DFB_ERR_ARG, "top_k %d outside [0, min(32, %d)]", a->top_k, a->n_vocab);
+    if (a->top_k > 0 && (!a->top_ids || !a->top_logprob)) return set_err(DFB_ERR_ARG, "null alternatives");
+    if ((a->logprob != nullptr) != (a->targets != nullptr)) return set_err(DFB_ERR_ARG, "targets and logprob go together");
+    if (!a->rows && a->n_rows > a->n_logits) return set_err(DFB_ERR_ARG, "%d rows of a matrix of %d", a->n_rows, a->n_logits);
+    if (a->n_rows == 0) return DFB_OK;
+    if (!a->logits || !aligned(a->logits, type_size(a->type))) return set_err(DFB_ERR_ARG, "logits null or not aligned to their type");
+    DeviceGuard g;
+    RET(g.enter(a->logits, "logits"));
+    int n_sm = 0;
+    RET(device_props(g.device(), &n_sm));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (a->type) {
+        case T_F32: logprobs_simple<float><<<a->n_rows, kLpThreads, 0, st>>>(*a, status); break;
+        case T_F16: logprobs_simple<__half><<<a->n_rows, kLpThreads, 0, st>>>(*a, status); break;
+        default: logprobs_simple<__nv_bfloat16><<<a->n_rows, kLpThreads, 0, st>>>(*a, status);
+    }
+    CK(cudaGetLastError());
+    return DFB_OK;
+}

@@ -205,6 +205,116 @@ int dfb_ctx_profile_read(dfb_ctx *c, dfb_prof_entry *out, int n);      /* n <= D
 int dfb_linear_noalloc(const dfb_model *m, int role, int layer, const void *x_f16_dev, int M, float *y_dev,
                        void *stream);
 
+/* ── operators on device tensors ──
+ * No counterpart in the reference (its cache is f32 and contiguous, diffuse-cache.h:14-147, and
+ * its sampler keeps no log probabilities).  Every pointer below is device memory of one GPU,
+ * owned by the caller, unless it says otherwise; the calls work on that GPU whatever the current
+ * device is, launch on `stream` (cudaStream_t as void*, NULL = legacy default stream) and return
+ * without waiting for it.  They allocate nothing, so they can be captured into a CUDA graph, and
+ * they hold no lock: calls on several streams or threads may overlap as long as they do not
+ * share a buffer that one of them writes (outputs, the cache pages written, a workspace).
+ *
+ * Values in device memory cannot be checked by the host.  A kernel that meets one it cannot use
+ * skips the access (it never reads or writes outside the tensors described to it) and ORs a bit
+ * into *status (one int32 the caller zeroes; NULL: not reported): */
+enum {
+    DFB_STAT_PAGE = 1,      /* a page id outside [0, n_pages): its rows / keys were left out */
+    DFB_STAT_POSITION = 2,  /* a position outside the page table or the rotation table, or not
+                               ascending: its row was left out; a length outside the page table */
+    DFB_STAT_ROWS = 4,      /* row_off not ascending within [0, n_rows], or more rows than max_rows */
+    DFB_STAT_NONFINITE = 8, /* K / V to be stored held NaN (stored as 0) or +-inf (stored as the largest code) */
+    DFB_STAT_TARGET = 16,   /* a target token >= n_vocab (its log probability is NaN), or a row index out of range */
+    DFB_STAT_LOGITS = 32    /* a logits row with NaN or +inf (its outputs are NaN, its ids -1) */
+};
+
+/* Element types of caller tensors (GGML ids): F32 0, F16 1, BF16 30. */
+
+/* A paged K/V cache in 8 bits.  A page holds `page` consecutive positions of one sequence, for
+ * every KV head: E4M3 codes [n_pages][n_kv][page][head_dim] for K and for V, and one f32 scale
+ * for each page and KV head (value = code * scale).  Position p of sequence s lies in page
+ * pages[s * max_pages + p / page].  head_dim 64 or 128; page 16, 32, 64 or 128.  k, v are
+ * 16-byte aligned.  The codes of positions behind a sequence's length are never used. */
+typedef struct {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    const int32_t *pages;
+    int32_t n_pages, n_kv, head_dim, page, n_seq, max_pages;
+} dfb_kv_cache;
+
+/* The rows one call of dfb_kv_append stores: sequence s has rows [row_off[s], row_off[s + 1]) of
+ * k and v ([n_rows][n_kv][head_dim], the last dimension contiguous, the other strides in
+ * elements).  They go to positions len[s], len[s] + 1, ... or, with pos, to pos[row] (strictly
+ * ascending within a sequence), where len[s] counts the positions that are already filled.
+ * rope: [n_rope][head_dim / 2] pairs (cos, sin), row = position: k is rotated by it (NEOX pairs
+ * (i, i + head_dim / 2), diffuse-graph.cpp:76-79) before it is stored; NULL: stored as it is.
+ * q, q_out: query rows [n_rows][n_q][head_dim] of the same positions, rotated into q_out (which
+ * may be q itself); NULL: none. */
+typedef struct {
+    const void *k, *v;
+    int32_t type;               /* of k, v, q and q_out */
+    int32_t n_rows, max_rows;   /* rows in all; most rows of any one sequence */
+    int64_t k_tok, k_head, v_tok, v_head;
+    const int32_t *row_off;     /* [n_seq + 1] */
+    const int32_t *len;         /* [n_seq] */
+    const int32_t *pos;         /* [n_rows] or NULL */
+    const float *rope;          /* or NULL */
+    int32_t n_rope;
+    int32_t n_q;
+    const void *q;              /* or NULL */
+    void *q_out;
+    int64_t q_tok, q_head, q_out_tok, q_out_head;
+} dfb_kv_rows;
+
+/* Store rows.  The scale of a (page, KV head) becomes the smallest power of two 2^e, e >= -64,
+ * with max |x| <= 448 * 2^e over the values the call writes there; while positions of that page
+ * below len[s] keep their values it does not shrink, and where it grows their codes are
+ * re-rounded once to the new scale.  Rows of different sequences must lie in different pages. */
+int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_t *status, void *stream);
+
+/* Attention of query rows over the cache: for each row and query head h,
+ * softmax(scale * q . K^T) V over the first n keys of its sequence, n = min(vis[row], len[s])
+ * (vis NULL: len[s]), KV head h / (n_q / n_kv) (diffuse-graph.cpp:97-119 over a stored cache).
+ * No key: the output row is 0 and its lse -inf. */
+typedef struct {
+    const void *q;              /* [n_rows][n_q][head_dim], last dimension contiguous */
+    void *out;                  /* same shape and type */
+    int32_t type;               /* F16 or BF16 */
+    int32_t n_q;
+    int32_t n_rows, max_rows, max_keys;  /* rows in all; bounds of any one sequence's rows and keys */
+    float scale;
+    int64_t q_tok, q_head, out_tok, out_head;
+    const int32_t *row_off;     /* [n_seq + 1] */
+    const int32_t *len;         /* [n_seq] keys */
+    const int32_t *vis;         /* [n_rows] or NULL */
+    float *lse;                 /* [n_rows][n_q] natural log of the softmax denominator, or NULL */
+} dfb_kv_attn;
+
+/* Bytes of workspace dfb_kv_attention needs for these sizes (the pointers are not looked at);
+ * 0 if none.  A call's workspace must not be used by another call that may run at the same time. */
+int dfb_kv_attention_workspace(const dfb_kv_cache *c, const dfb_kv_attn *a, size_t *bytes);
+int dfb_kv_attention(const dfb_kv_cache *c, const dfb_kv_attn *a, void *workspace, size_t ws_bytes, int32_t *status,
+                     void *stream);
+
+/* Log probabilities of given tokens under softmax(logits), the entropy of the distribution (nats)
+ * and the top_k most probable tokens with theirs, for n_rows rows of a logits matrix
+ * [n_logits][n_vocab] of row stride ld (elements); rows: the matrix row of each (NULL: row i).
+ * Equal logits rank by the lower id.  targets[i] < 0: logprob 0 (no token asked for); targets
+ * NULL with logprob NULL.  A row of -inf alone has entropy 0 and log probabilities -inf. */
+typedef struct {
+    const void *logits;
+    int32_t type;               /* F32, F16 or BF16 */
+    int32_t n_vocab, n_rows, n_logits;
+    int64_t ld;
+    const int32_t *rows;        /* [n_rows] or NULL */
+    const int32_t *targets;     /* [n_rows] or NULL */
+    float *logprob;             /* [n_rows] or NULL */
+    float *entropy;             /* [n_rows] or NULL */
+    int32_t top_k;              /* 0..32, at most n_vocab */
+    int32_t *top_ids;           /* [n_rows][top_k] */
+    float *top_logprob;         /* [n_rows][top_k] */
+} dfb_logprob_args;
+int dfb_token_logprobs(const dfb_logprob_args *a, int32_t *status, void *stream);
+
 /* Device stream of a context (cudaStream_t as void*), for callers that time it. */
 int dfb_ctx_stream(dfb_ctx *c, void **stream);
 
