@@ -1,8 +1,10 @@
 // Entry points of the operators on device tensors (include/diffuse_b200.h): argument checks, the
 // choice of a kernel variant, launches.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <cmath>
@@ -73,6 +75,7 @@ int check_cache(const dfb_kv_cache *c) {
     if (c->n_pages <= 0 || c->n_kv <= 0 || c->n_seq <= 0 || c->max_pages <= 0)
         return set_err(DFB_ERR_ARG, "cache of %d pages, %d KV heads, %d sequences of %d pages", c->n_pages, c->n_kv, c->n_seq, c->max_pages);
     if (c->n_seq > 65535 || c->n_kv > 8192) return set_err(DFB_ERR_UNSUPPORTED, "%d sequences / %d KV heads", c->n_seq, c->n_kv);
+    if ((int64_t)c->n_pages * c->n_kv * c->page > INT32_MAX) return set_err(DFB_ERR_UNSUPPORTED, "pool of %d pages of %d heads", c->n_pages, c->n_kv);
     if ((int64_t)c->max_pages * c->page > INT32_MAX) return set_err(DFB_ERR_UNSUPPORTED, "page table of %d pages", c->max_pages);
     if (!aligned(c->k, 16) || !aligned(c->v, 16)) return set_err(DFB_ERR_ARG, "cache codes not 16-byte aligned");
     return DFB_OK;
@@ -101,10 +104,87 @@ int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, bool vec, dim3 grid, i
     return DFB_OK;
 }
 
-template <typename T, int HD>
-int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, int32_t *status, cudaStream_t st) {
-    kv_attn_simple<T, HD><<<dim3((a.max_rows + 3) / 4, a.n_q, c.n_seq), 128, 0, st>>>(c, a, status);
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        cudaDriverEntryPointQueryResult q;
+        void *p = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }();
+    return fn;
+}
+// The cache's codes as a matrix of head_dim-byte rows, copied in boxes of at most kKeyTile
+// positions of one page, swizzled over the row length.
+int code_map(CUtensorMap *m, void *codes, const dfb_kv_cache &c) {
+    const auto fn = tensor_map_encoder();
+    if (!fn) return set_err(DFB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[2] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.n_pages * c.n_kv * c.page};
+    const cuuint64_t strides[1] = {(cuuint64_t)c.head_dim};
+    const cuuint32_t box[2] = {(cuuint32_t)c.head_dim, (cuuint32_t)std::min(c.page, kKeyTile)}, es[2] = {1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_err(DFB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return DFB_OK;
+}
+
+// How one call is cut up: rows per CTA, and parts of the key axis where the row tiles alone would
+// leave SMs idle.
+struct AttnPlan {
+    int rows, tiles, splits;
+};
+AttnPlan attn_plan(const dfb_kv_cache &c, const dfb_kv_attn &a, int n_sm) {
+    AttnPlan p;
+    const int64_t packed = (int64_t)a.max_rows * (a.n_q / c.n_kv);
+    p.rows = packed <= 16 ? 16 : packed <= 32 ? 32 : packed <= 64 ? 64 : 128;
+    p.tiles = (int)((packed + p.rows - 1) / p.rows);
+    const int64_t base = (int64_t)p.tiles * c.n_kv * c.n_seq, key_tiles = (a.max_keys + kKeyTile - 1) / kKeyTile;
+    const int64_t want = 2 * n_sm / std::max<int64_t>(base, 1);
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, key_tiles / 4, 128}));
+    return p;
+}
+size_t attn_ws_bytes(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p) {
+    return p.splits == 1 ? 0 : (size_t)p.splits * a.n_rows * a.n_q * (c.head_dim + 1) * sizeof(float);
+}
+
+template <typename T, int HD, int MW, int KW>
+int attn_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, const AttnParts &parts, const CUtensorMap &tk,
+                const CUtensorMap &tv, bool vec, int dev, int32_t *status, cudaStream_t st) {
+    const auto kern = kv_attn_kernel<T, HD, MW, KW>;
+    constexpr int smem = KvSmem<HD, MW, KW>::bytes;
+    static bool attr_set[64] = {false};
+    if (!attr_set[dev]) {
+        CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        attr_set[dev] = true;
+    }
+    kern<<<dim3(p.tiles * p.splits, c.n_kv, c.n_seq), (MW * KW + 1) * 32, smem, st>>>(c, a, tk, tv, parts, vec, status);
     CK(cudaGetLastError());
+    return DFB_OK;
+}
+
+template <typename T, int HD>
+int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float *ws, int dev, int32_t *status, cudaStream_t st) {
+    CUtensorMap tk, tv;
+    RET(code_map(&tk, c.k, c));
+    RET(code_map(&tv, c.v, c));
+    const bool vec = vec_ok(a.q, a.type, a.q_tok, a.q_head) && vec_ok(a.out, a.type, a.out_tok, a.out_head);
+    AttnParts parts;
+    parts.splits = p.splits;
+    if (p.splits > 1) {
+        parts.o = ws;
+        parts.w = ws + (size_t)p.splits * a.n_rows * a.n_q * HD;
+    }
+    switch (p.rows) {
+        case 16: RET((attn_launch<T, HD, 1, 4>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
+        case 32: RET((attn_launch<T, HD, 2, 4>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
+        case 64: RET((attn_launch<T, HD, 4, 2>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
+        default: RET((attn_launch<T, HD, 8, 1>(c, a, p, parts, tk, tv, vec, dev, status, st)));
+    }
+    if (p.splits > 1) {
+        const int64_t per_seq = (int64_t)a.max_rows * a.n_q;
+        CK(launch_k(kv_attn_join_kernel<T, HD>, dim3((unsigned)((per_seq + 256 / (HD / 8) - 1) / (256 / (HD / 8))), c.n_seq), dim3(256), 0, st,
+                    true, c, a, parts, vec));
+    }
     return DFB_OK;
 }
 
@@ -113,7 +193,7 @@ int check_attn(const dfb_kv_cache *c, const dfb_kv_attn *a) {
     if (!a) return set_err(DFB_ERR_ARG, "null arguments");
     if (a->type != T_F16 && a->type != T_BF16) return set_err(DFB_ERR_UNSUPPORTED, "query type %d not supported (F16 / BF16)", a->type);
     if (a->n_q <= 0 || a->n_q % c->n_kv) return set_err(DFB_ERR_ARG, "%d query heads over %d KV heads", a->n_q, c->n_kv);
-    if (a->n_q > 65535) return set_err(DFB_ERR_UNSUPPORTED, "%d query heads", a->n_q);
+    if (a->n_q > 65535 || (int64_t)a->max_rows * a->n_q > INT32_MAX) return set_err(DFB_ERR_UNSUPPORTED, "%d query heads of %d rows", a->n_q, a->max_rows);
     if (a->n_rows < 0 || a->max_rows < 0 || a->max_keys < 0) return set_err(DFB_ERR_ARG, "negative size");
     if (!std::isfinite(a->scale)) return set_err(DFB_ERR_ARG, "scale must be finite");
     return DFB_OK;
@@ -156,6 +236,13 @@ extern "C" int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_
 extern "C" int dfb_kv_attention_workspace(const dfb_kv_cache *c, const dfb_kv_attn *a, size_t *bytes) {
     if (!bytes) return set_err(DFB_ERR_ARG, "null pointer");
     *bytes = 0;
+    RET(check_attn(c, a));
+    if (a->n_rows == 0 || a->max_rows == 0) return DFB_OK;
+    DeviceGuard g;
+    RET(g.enter(c->k, "the cache"));
+    int n_sm = 0;
+    RET(device_props(g.device(), &n_sm));
+    *bytes = attn_ws_bytes(*c, *a, attn_plan(*c, *a, n_sm));
     return DFB_OK;
 }
 
@@ -170,9 +257,17 @@ extern "C" int dfb_kv_attention(const dfb_kv_cache *c, const dfb_kv_attn *a, voi
     RET(g.enter(c->k, "the cache"));
     int n_sm = 0;
     RET(device_props(g.device(), &n_sm));
+    const AttnPlan p = attn_plan(*c, *a, n_sm);
+    const size_t need = attn_ws_bytes(*c, *a, p);
+    if (need && (!workspace || ws_bytes < need || !aligned(workspace, 16)))
+        return set_err(DFB_ERR_ARG, "workspace of %zu bytes at %p, need %zu 16-byte aligned", ws_bytes, workspace, need);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->type == T_F16) return c->head_dim == 64 ? attn_t<__half, 64>(*c, *a, status, st) : attn_t<__half, 128>(*c, *a, status, st);
-    return c->head_dim == 64 ? attn_t<__nv_bfloat16, 64>(*c, *a, status, st) : attn_t<__nv_bfloat16, 128>(*c, *a, status, st);
+    float *ws = static_cast<float *>(workspace);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        return c->head_dim == 64 ? attn_t<T, 64>(*c, *a, p, ws, g.device(), status, st) : attn_t<T, 128>(*c, *a, p, ws, g.device(), status, st);
+    };
+    return a->type == T_F16 ? go(__half()) : go(__nv_bfloat16());
 }
 
 extern "C" int dfb_token_logprobs(const dfb_logprob_args *a, int32_t *status, void *stream) {

@@ -15,7 +15,7 @@ import torch
 
 from . import BF16, F16, F32, DiffuseError, native
 
-(STAT_PAGE, STAT_POSITION, STAT_ROWS, STAT_NONFINITE, STAT_TARGET, STAT_LOGITS) = (1, 2, 4, 8, 16, 32)
+(STAT_PAGE, STAT_POSITION, STAT_ROWS, STAT_NONFINITE, STAT_TARGET, STAT_LOGITS, STAT_TIMEOUT) = (1, 2, 4, 8, 16, 32, 64)
 
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _P, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
