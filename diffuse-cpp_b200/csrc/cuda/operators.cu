@@ -13,6 +13,7 @@
 #include "host_util.h"
 #include "kv_append.cuh"
 #include "kv_attention.cuh"
+#include "kv_attention_tc.cuh"
 #include "logprobs.cuh"
 
 using namespace dfb;
@@ -136,10 +137,10 @@ struct AttnPlan {
 AttnPlan attn_plan(const dfb_kv_cache &c, const dfb_kv_attn &a, int n_sm) {
     AttnPlan p;
     const int64_t packed = (int64_t)a.max_rows * (a.n_q / c.n_kv);
-    p.rows = packed <= 16 ? 16 : packed <= 32 ? 32 : packed <= 64 ? 64 : 128;
+    p.rows = packed <= 16 ? 16 : packed <= 32 ? 32 : packed <= 64 ? 64 : kTcRows;
     p.tiles = (int)((packed + p.rows - 1) / p.rows);
     const int64_t base = (int64_t)p.tiles * c.n_kv * c.n_seq, key_tiles = (a.max_keys + kKeyTile - 1) / kKeyTile;
-    const int64_t want = 2 * n_sm / std::max<int64_t>(base, 1);
+    const int64_t want = (p.rows == kTcRows ? 1 : 2) * n_sm / std::max<int64_t>(base, 1);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, key_tiles / 4, 128}));
     return p;
 }
@@ -163,6 +164,22 @@ int attn_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, 
 }
 
 template <typename T, int HD>
+int attn_tc_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, const AttnParts &parts, const CUtensorMap &tk,
+                   const CUtensorMap &tv, bool vec, int dev, int32_t *status, cudaStream_t st) {
+    const auto kern = kv_attn_tc_kernel<T, HD>;
+    constexpr int smem = TcSmem<HD>::bytes;
+    static_assert(smem <= 232448, "shared memory of one CTA");
+    static bool attr_set[64] = {false};
+    if (!attr_set[dev]) {
+        CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        attr_set[dev] = true;
+    }
+    kern<<<dim3(p.tiles * p.splits, c.n_kv, c.n_seq), kTcThreads, smem, st>>>(c, a, tk, tv, parts, vec, status);
+    CK(cudaGetLastError());
+    return DFB_OK;
+}
+
+template <typename T, int HD>
 int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float *ws, int dev, int32_t *status, cudaStream_t st) {
     CUtensorMap tk, tv;
     RET(code_map(&tk, c.k, c));
@@ -178,7 +195,7 @@ int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float
         case 16: RET((attn_launch<T, HD, 1, 4>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
         case 32: RET((attn_launch<T, HD, 2, 4>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
         case 64: RET((attn_launch<T, HD, 4, 2>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
-        default: RET((attn_launch<T, HD, 8, 1>(c, a, p, parts, tk, tv, vec, dev, status, st)));
+        default: RET((attn_tc_launch<T, HD>(c, a, p, parts, tk, tv, vec, dev, status, st)));
     }
     if (p.splits > 1) {
         const int64_t per_seq = (int64_t)a.max_rows * a.n_q;
