@@ -29,7 +29,7 @@ struct TcSmem {
     static constexpr int raw = kTcKeys * HD;
     static constexpr int q_off = 0, slot_off = 2 * q, raw_off = slot_off + kTcSlots * slot, sc_off = raw_off + kTcRaw * raw;
     static constexpr int bar_off = sc_off + 4 * 8 * 16;
-    static constexpr int n_bars = 2 * kTcRaw + 2 * kTcSlots + 8;
+    static constexpr int n_bars = 2 * kTcRaw + kTcSlots + 12;
     static constexpr int bytes = 1024 + bar_off + n_bars * 8 + 32;
 };
 
@@ -77,6 +77,23 @@ __device__ __forceinline__ void tmem_ld_wait32(float *r) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(d)
+        : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)), "l"(*reinterpret_cast<const uint64_t *>(&c)));
+    return *reinterpret_cast<const float2 *>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)));
+    return *reinterpret_cast<const float2 *>(&d);
+}
+// The factor of a score is kept above 0, so that a masked score of -inf stays -inf where the softmax
+// scale is 0 or the product of the scales underflows; every score times this is 0 beside an exponent.
+constexpr float kMinFactor = 1.1754944e-38f;
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -113,10 +130,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     using L = TcSmem<HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    float4 *sc = reinterpret_cast<float4 *>(sm + L::sc_off);  // [tile & 3][8 runs of 16 keys] ks, log2 vs, 1 / vs
+    float4 *sc = reinterpret_cast<float4 *>(sm + L::sc_off);  // [tile & 3][8 runs of 16 keys] ks, log2 vs, 1 / vs, any absent
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + L::bar_off);
-    uint64_t *raw_full = bars, *raw_empty = raw_full + kTcRaw, *conv_full = raw_empty + kTcRaw, *conv_empty = conv_full + kTcSlots;
-    uint64_t *bar_s = conv_empty + kTcSlots, *bar_p = bar_s + 2, *bar_o = bar_p + 2, *bar_q = bar_o + 2, *bar_drain = bar_q + 1;
+    uint64_t *raw_full = bars, *raw_empty = raw_full + kTcRaw, *conv_full = raw_empty + kTcRaw, *freed = conv_full + kTcSlots;
+    uint64_t *bar_s = freed + 2, *bar_pa = bar_s + 2, *bar_pb = bar_pa + 2, *bar_o = bar_pb + 2, *bar_q = bar_o + 2, *bar_drain = bar_q + 1;
     int *shared_i = reinterpret_cast<int *>(bars + L::n_bars);  // abort flag, most keys of a row, TMEM address
     volatile int *abort_flag = shared_i;
 
@@ -136,11 +153,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         for (int i = 0; i < kTcSlots; i++) {
             mbar_init(&conv_full[i], 4);
-            mbar_init(&conv_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(&bar_s[i], 1);
-            mbar_init(&bar_p[i], 4);
+            mbar_init(&bar_pa[i], 4);
+            mbar_init(&bar_pb[i], 4);
+            mbar_init(&freed[i], 1);
             mbar_init(&bar_o[i], 1);
         }
         mbar_init(bar_q, two ? 8 : 4);
@@ -169,35 +187,52 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         setmaxnreg_inc<184>();
         const int w = warp >> 2;
         if (w == 0 || two) {
-            // ── queries: this thread's row as f16, scaled by a power of two ──
-            const int tok = sq.r0 + (live ? R / rep : 0), head = kvh * rep + (live ? R % rep : 0);
+            // ── queries: the warp's 32 rows as f16, scaled by a power of two ──
+            constexpr int LPR = HD / 8, RPI = 32 / LPR;  // lanes of a row (16 bytes each), rows of one load
             const uint32_t tm_s = tmem + w * 128 + ((uint32_t)(warp & 3) << 21), tm_o = tmem + 256 + w * 128 + ((uint32_t)(warp & 3) << 21);
-            float cr = a.scale * kLog2e;
-            {
-                const T *q = reinterpret_cast<const T *>(a.q) + tok * a.q_tok + head * a.q_head;
-                float up = 1.f;
-                if constexpr (!std::is_same<T, __half>::value) {
-                    float mx = 0.f;
-                    if (live)
-                        for (int d = 0; d < HD; d += 8) {
-                            float x[8];
-                            load8(q + d, vec, x);
+            const int wrow = row0 + warp * 32;  // the warp's first packed row
+            uint8_t *stage = sm + L::q_off + w * L::q + (warp & 3) * 32 * (HD * 2);
+            float cr = fabsf(a.scale) * kLog2e;
+            if (nt > 0) {  // (without keys the output goes through this memory right away)
+                uint4 raw[LPR];
+                const int ch = lane % LPR, sub = lane / LPR;
 #pragma unroll
-                            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
-                        }
-                    const int e = (int)(__float_as_uint(mx) >> 23) - 127;
-                    if (mx > 0.f && mx < INFINITY) up = exp2i(max(-e, -126));
-                    cr *= 1.f / up;
+                for (int i = 0; i < LPR; i++) {
+                    const int r = wrow + i * RPI + sub;
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (r < n_packed) {
+                        const T *q = reinterpret_cast<const T *>(a.q) + (sq.r0 + r / rep) * a.q_tok + (kvh * rep + r % rep) * a.q_head + 8 * ch;
+                        if (vec) raw[i] = *reinterpret_cast<const uint4 *>(q);
+                        else
+#pragma unroll
+                            for (int e = 0; e < 8; e++) reinterpret_cast<T *>(&raw[i])[e] = q[e];
+                    }
                 }
-                uint8_t *dst = sm + L::q_off + w * L::q + (tid & 127) * 128;
-                for (int d = 0; d < HD; d += 8) {
-                    float x[8] = {};
-                    if (live) load8(q + d, vec, x);
+                float mine = 1.f;
+#pragma unroll
+                for (int i = 0; i < LPR; i++) {
+                    float x[8], up = 1.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = to_f32<T>(reinterpret_cast<const T *>(&raw[i])[e]);
+                    if constexpr (!std::is_same<T, __half>::value) {
+                        float mx = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
+#pragma unroll
+                        for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const int e = (int)(__float_as_uint(mx) >> 23) - 127;
+                        if (mx > 0.f && mx < INFINITY) up = exp2i(min(max(-e, -126), 60));
+                        const float got = __shfl_sync(0xffffffffu, up, (lane % RPI) * LPR);  // of row i * RPI + lane % RPI
+                        if (lane / RPI == i) mine = got;
+                    }
+                    up = a.scale < 0.f ? -up : up;  // a negative scale turns q's sign: the factors of the scores stay positive
                     uint4 u;
                     u.x = pack_f16(x[0] * up, x[1] * up); u.y = pack_f16(x[2] * up, x[3] * up);
                     u.z = pack_f16(x[4] * up, x[5] * up); u.w = pack_f16(x[6] * up, x[7] * up);
-                    *reinterpret_cast<uint4 *>(dst + (d / 64) * 16384 + (((d / 8 & 7) ^ (tid & 7)) << 4)) = u;
+                    const int r = (warp & 3) * 32 + i * RPI + sub;
+                    *reinterpret_cast<uint4 *>(sm + L::q_off + w * L::q + (ch / 8) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = u;
                 }
+                cr *= 1.f / mine;
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_q);
@@ -206,6 +241,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             float M = -INFINITY, l = 0.f;
             for (int j = 0; j < nt; j++) {
                 if (!attn_wait(&bar_s[w], j & 1, abort_flag)) break;
+                if (wrow >= n_packed) {  // no row of this warp exists: whatever its lanes of P hold, no one reads what comes of it
+                    if (lane == 0) {
+                        mbar_arrive(&bar_pa[w]);
+                        mbar_arrive(&bar_pb[w]);
+                    }
+                    continue;
+                }
                 tc_fence_after();
                 float x[128];
 #pragma unroll
@@ -214,20 +256,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int i = 0; i < 4; i++) tmem_ld_wait32(x + 32 * i);
                 const float4 *g = sc + (j & 3) * 8;
                 const int left = nr - (t0 + j) * kTcKeys;  // keys of the tile this row sees
-                float mx = -INFINITY;
+                const bool holes = g[0].w != 0.f;
+                // rows that see only a part of the tile, keys of a bad page: rare
+                if (__any_sync(0xffffffffu, left < kTcKeys || holes)) {
 #pragma unroll
-                for (int p = 0; p < 8; p++) {
-                    const float4 f = g[p];
-                    const float fk = cr * f.x;
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[16 * p + e] = fmaf(x[16 * p + e], fk, f.y);
-                    if (left < 16 * (p + 1) || f.y == -INFINITY) {
+                    for (int p = 0; p < 8; p++) {
+                        const bool none = g[p].y == -INFINITY;
 #pragma unroll
                         for (int e = 0; e < 16; e++)
-                            if (16 * p + e >= left || f.y == -INFINITY) x[16 * p + e] = -INFINITY;
+                            if (16 * p + e >= left || none) x[16 * p + e] = -INFINITY;
                     }
+                }
+                // the largest t = s fk + lv of the tile: by runs, whose factor is not negative
+                float mx = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) mx = fmaxf(mx, x[16 * p + e]);
+                for (int p = 0; p < 8; p += 2) {
+                    const float4 f = g[p], f1 = g[p + 1];
+                    float m[4];
+#pragma unroll
+                    for (int h = 0; h < 4; h++) {
+                        const float *y = x + 16 * p + 8 * h;
+                        m[h] = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), fmaxf(y[6], y[7]));
+                    }
+                    mx = max3(mx, fmaf(fmaxf(m[0], m[1]), fmaxf(cr * f.x, kMinFactor), f.y), fmaf(fmaxf(m[2], m[3]), fmaxf(cr * f1.x, kMinFactor), f1.y));
                 }
                 mx -= kTcOff;
                 // follow the maximum only by jumps: most tiles leave O as it is
@@ -257,21 +308,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     uint32_t u[16];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float sum = 0.f;
+                        const float4 f = g[p + h];
+                        const float fk = fmaxf(cr * f.x, kMinFactor), add = f.y - base;
+                        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            const float p0 = ex2(x[16 * (p + h) + e] - base), p1 = ex2(x[16 * (p + h) + e + 1] - base);
-                            sum += p0 + p1;
-                            u[8 * h + e / 2] = pack_f16(p0, p1);
+                            const float2 y = fma2(make_float2(x[16 * (p + h) + e], x[16 * (p + h) + e + 1]), make_float2(fk, fk), make_float2(add, add));
+                            const float2 pr = make_float2(ex2(y.x), ex2(y.y));
+                            sum = add2(sum, pr);
+                            u[8 * h + e / 2] = pack_f16(pr.x, pr.y);
                         }
-                        l = fmaf(sum, g[p + h].z, l);
+                        l = fmaf(sum.x + sum.y, f.z, l);
                     }
                     tmem_st16(tm_s + 8 * p, u);
+                    if (p == 2 || p == 6) {  // each half of the tile's keys on its own: its P V starts under the other's exponentials
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p == 2 ? &bar_pa[w] : &bar_pb[w]);
+                    }
                 }
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_p[w]);
             }
             // ── output ──
             bool ok = true;
@@ -279,19 +335,58 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
             if (!ok && status) atomicOr(status, DFB_STAT_TIMEOUT);
             const float inv = l > 0.f ? 1.f / l : 0.f, lw = l > 0.f ? M + log2f(l) : -INFINITY;
+            // through the warp's part of the query tile (its last reader was the last score MMA), so that
+            // rows leave as whole 16-byte columns of consecutive lanes
+            const int own = wrow + lane;  // this thread's packed row
+            if (own < n_packed) {
+                const size_t row = (size_t)(sq.r0 + own / rep) * a.n_q + kvh * rep + own % rep;
+                if (parts.o) parts.w[(size_t)split * a.n_rows * a.n_q + row] = lw;
+                else if (a.lse) a.lse[row] = lw * kLn2;
+            }
+            auto put = [&](auto zero, int pass) {  // zero's type: of the stored elements
+                using E = decltype(zero);
+                constexpr int PER = 16 / sizeof(E), N = HD * 2 / sizeof(E);  // elements of a column, of a pass
 #pragma unroll
-            for (int i = 0; i < HD / 32; i++) {
-                float o[32];
-                if (nt > 0) {
-                    tmem_ld32(tm_o + 32 * i, o);
-                    tmem_ld_wait32(o);
+                for (int i = 0; i < N / 32; i++) {
+                    float o[32];
+                    if (nt > 0) {
+                        tmem_ld32(tm_o + pass * N + 32 * i, o);
+                        tmem_ld_wait32(o);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 32 / PER; h++) {
+                        E t[PER];
+#pragma unroll
+                        for (int e = 0; e < PER; e++) t[e] = from_f32<E>(l > 0.f ? o[PER * h + e] * inv : 0.f);
+                        const int ch = i * (32 / PER) + h;
+                        *reinterpret_cast<uint4 *>(stage + lane * (HD * 2) + ((ch ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(t);
+                    }
                 }
+                __syncwarp();
+                const int ch = lane % LPR;
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[e] = l > 0.f ? o[e] * inv : 0.f;
-                if (live)
+                for (int i = 0; i < LPR; i++) {
+                    const int r = i * RPI + lane / LPR, R = wrow + r;
+                    const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * (HD * 2) + ((ch ^ (r & 7)) << 4));
+                    if (R >= n_packed) continue;
+                    const int tok = sq.r0 + R / rep, head = kvh * rep + R % rep;
+                    E *dst = sizeof(E) == 4 ? reinterpret_cast<E *>(parts.o) + ((size_t)split * a.n_rows * a.n_q + (size_t)tok * a.n_q + head) * HD
+                                            : reinterpret_cast<E *>(a.out) + tok * a.out_tok + head * a.out_head;
+                    dst += pass * N + ch * PER;
+                    if (sizeof(E) == 4 || vec) *reinterpret_cast<uint4 *>(dst) = u;
+                    else
 #pragma unroll
-                    for (int h = 0; h < 4; h++)
-                        attn_store<T, HD>(a, parts, split, tok, head, 32 * i + 8 * h, reinterpret_cast<float(&)[8]>(o[8 * h]), lw, vec);
+                        for (int e = 0; e < PER; e++) dst[e] = reinterpret_cast<const E *>(&u)[e];
+                }
+                __syncwarp();
+            };
+            if (wrow < n_packed) {
+                if (parts.o) {
+                    put(0.f, 0);
+                    put(0.f, 1);
+                } else {
+                    put(T(0.f), 0);
+                }
             }
             tc_fence_before();
         }
@@ -303,7 +398,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int n = 0; n < 2 * nt; n++) {
                 const int rs = n % kTcRaw, cs = n % kTcSlots, j = n >> 1;
                 if (!attn_wait(&raw_full[rs], (n / kTcRaw) & 1, abort_flag)) break;
-                if (n >= kTcSlots && !attn_wait(&conv_empty[cs], (n / kTcSlots - 1) & 1, abort_flag)) break;
+                // V(j) and K(j + 1) are freed together, by event j + 1 (K(0) by event 0); events alternate
+                // between two barriers, and the issuer is never two events ahead of this wait
+                const int ev = (n - kTcSlots + 1) >> 1;
+                if (n >= kTcSlots && !attn_wait(&freed[ev & 1], (ev >> 1) & 1, abort_flag)) break;
                 const uint8_t *src = sm + L::raw_off + rs * L::raw;
                 uint8_t *dst = sm + L::slot_off + cs * L::slot;
                 const float4 *g = sc + (j & 3) * 8;
@@ -348,19 +446,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (lane == 0 && nt > 0) {
                 const uint32_t id_s = idesc_f16(128, kTcKeys), id_o = idesc_f16(128, HD) | (1u << 16);  // V is MN-major
                 const uint32_t base = smem_u32(sm);
+                const uint64_t dq = sw128_desc(base + L::q_off), dk = sw128_desc(base + L::slot_off), dv = mn128_desc(base + L::slot_off, 16384);
                 auto score = [&](int w, int n) {
-                    const uint64_t da = sw128_desc(base + L::q_off + w * L::q), db = sw128_desc(base + L::slot_off + (n % kTcSlots) * L::slot);
+                    const uint64_t da = dq + w * (L::q >> 4), db = dk + (n % kTcSlots) * (L::slot >> 4);
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++) {
                         const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
                         mma1_f16_ss(tmem + w * 128, da + off, db + off, id_s, k > 0);
                     }
                 };
-                auto value = [&](int w, int n, bool first) {
-                    const uint64_t db = mn128_desc(base + L::slot_off + (n % kTcSlots) * L::slot, 16384);
+                auto value = [&](int w, int n, int half, bool add) {
+                    const uint64_t db = dv + (n % kTcSlots) * (L::slot >> 4);
 #pragma unroll
-                    for (int k = 0; k < kTcKeys / 16; k++)
-                        mma1_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + 8 * k, db + (2048 >> 4) * k, id_o, !(first && k == 0));
+                    for (int i = 0; i < kTcKeys / 32; i++) {
+                        const int k = half * (kTcKeys / 32) + i;
+                        mma1_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + 8 * k, db + (2048 >> 4) * k, id_o, add || i > 0);
+                    }
                 };
                 auto ready = [&](uint64_t *b, int ph) {
                     const bool ok = thread_wait(b, ph, abort_flag);
@@ -376,15 +477,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         score(1, 0);
                         mma1_commit(&bar_s[1]);
                     }
-                    mma1_commit(&conv_empty[0]);
+                    mma1_commit(&freed[0]);
                 }
                 for (int j = 0; ok && j < nt; j++) {
                     const int nv = 2 * j + 1, nk = 2 * j + 2;
                     const bool more = j + 1 < nt;
                     ok = filled(nv);
                     for (int w = 0; ok && w < (two ? 2 : 1); w++) {
-                        if (!(ok = ready(&bar_p[w], j & 1))) break;
-                        value(w, nv, j == 0);
+                        if (!(ok = ready(&bar_pa[w], j & 1))) break;
+                        value(w, nv, 0, j > 0);
+                        if (!(ok = ready(&bar_pb[w], j & 1))) break;
+                        value(w, nv, 1, true);
                         if (!more) mma1_commit(&bar_o[w]);
                         else {
                             if (w == 0 && !(ok = filled(nk))) break;
@@ -392,10 +495,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             mma1_commit(&bar_s[w]);
                         }
                     }
-                    if (ok && more) {  // (the last commit is bar_o's, which the softmax warps wait for)
-                        mma1_commit(&conv_empty[nv % kTcSlots]);
-                        mma1_commit(&conv_empty[nk % kTcSlots]);
-                    }
+                    if (ok && more) mma1_commit(&freed[(j + 1) & 1]);  // (the last commit is bar_o's, which the softmax warps wait for)
                 }
                 if (!ok) {  // let what was issued end before TMEM is freed
                     mma1_commit(bar_drain);
@@ -442,7 +542,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const int src = b0 + (lane & 7) * 16 / box;
                     const int gp = __shfl_sync(0xffffffffu, pid, src);
                     const float gk = __shfl_sync(0xffffffffu, ks, src), gv = __shfl_sync(0xffffffffu, vs, src);
-                    if (lane < 8) sc[(j & 3) * 8 + lane] = make_float4(gk, gp < 0 ? -INFINITY : log2f(gv), 1.f / gv, 0.f);
+                    const bool holes = __any_sync(0xffffffffu, gp < 0);
+                    if (lane < 8) sc[(j & 3) * 8 + lane] = make_float4(gk, gp < 0 ? -INFINITY : log2f(gv), 1.f / gv, holes ? 1.f : 0.f);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&raw_full[rs], n_ok * box * HD);
