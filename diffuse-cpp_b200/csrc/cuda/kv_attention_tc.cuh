@@ -1,12 +1,13 @@
 // Attention over the paged 8-bit cache for many query rows: tcgen05 MMAs on tiles of 2 x 128 packed
 // rows x 128 keys (arithmetic: kv_attention.cuh).
 //
-// One CTA (16 warps) works on one sequence, KV head and tile of 256 packed rows:
-//   warps 0-3, 4-7  softmax of row tile 0 / 1, one row per thread (TMEM lane): scores from TMEM,
-//                   p' back into their place as f16 (the A operand of P V), rare rescales of O
-//   warps 8-11      converters: E4M3 codes -> f16 operands in shared memory, both of K and of V as
+// One CTA (22 warps) works on one sequence, KV head and tile of 256 packed rows:
+//   warps 0-7, 8-15 softmax of row tile 0 / 1, two threads to a row (TMEM lane), 64 keys each: scores
+//                   from TMEM, p' back into their place as f16 (the A operand of P V), rare rescales
+//                   of O
+//   warps 16-19     converters: E4M3 codes -> f16 operands in shared memory, both of K and of V as
 //                   rows of 64 dimensions swizzled over 128 bytes (K-major for K, MN-major for V)
-//   warp 12         MMA issuer, warp 13 loader (one tensor copy per run of page positions)
+//   warp 20         MMA issuer, warp 21 loader (one tensor copy per run of page positions)
 // MMA order: S0(0) S1(0), then for each key tile j: P0 V, S0(j+1), P1 V, S1(j+1), so one row tile's
 // softmax runs under the other's MMAs; S0(j+1) is complete only after P0 V(j), so a softmax thread
 // that has its scores may rescale its row of O without another wait.
@@ -17,7 +18,7 @@ namespace dfb {
 
 constexpr int kTcKeys = 128;     // keys of one tile
 constexpr int kTcRows = 256;     // packed rows of one CTA
-constexpr int kTcThreads = 512;
+constexpr int kTcThreads = 704;
 constexpr int kTcRaw = 2;        // raw slots: 128 x HD codes of K or V
 constexpr int kTcSlots = 4;      // f16 slots, K and V of successive tiles in turn
 constexpr float kTcOff = 7.f, kTcSlack = 8.f;  // p' <= 2^(off + slack) = 2^15 although the maximum is only followed by jumps
@@ -30,7 +31,8 @@ struct TcSmem {
     static constexpr int q_off = 0, slot_off = 2 * q, raw_off = slot_off + kTcSlots * slot, sc_off = raw_off + kTcRaw * raw;
     static constexpr int bar_off = sc_off + 4 * 8 * 16;
     static constexpr int n_bars = 2 * kTcRaw + kTcSlots + 12;
-    static constexpr int bytes = 1024 + bar_off + n_bars * 8 + 32;
+    static constexpr int crow_off = bar_off + n_bars * 8 + 32;
+    static constexpr int bytes = 1024 + crow_off + kTcRows * 4;
 };
 
 __device__ __forceinline__ void tmem_alloc1(uint32_t *holder, uint32_t ncols) {
@@ -94,10 +96,16 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // The factor of a score is kept above 0, so that a masked score of -inf stays -inf where the softmax
 // scale is 0 or the product of the scales underflows; every score times this is 0 beside an exponent.
 constexpr float kMinFactor = 1.1754944e-38f;
-template <int N>
-__device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Whether any of the n threads of a named barrier passes true.
+__device__ __forceinline__ bool named_bar_any(uint32_t id, uint32_t n, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.or.aligned.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(n), "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
 // Bounded wait of one thread (the MMA issuer and single waits); see attn_wait.
 __device__ __forceinline__ bool thread_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -161,19 +169,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&freed[i], 1);
             mbar_init(&bar_o[i], 1);
         }
-        mbar_init(bar_q, two ? 8 : 4);
+        mbar_init(bar_q, two ? 16 : 8);
         mbar_init(bar_drain, 1);
         fence_barrier_init();
     }
-    if (warp == 12) tmem_alloc1(reinterpret_cast<uint32_t *>(&shared_i[2]), 512);
+    if (warp == 20) tmem_alloc1(reinterpret_cast<uint32_t *>(&shared_i[2]), 512);
     __syncthreads();
     // keys the tile's rows see
-    const int R = row0 + tid;  // this thread's packed row (softmax warps)
-    const bool live = tid < kTcRows && R < n_packed;
+    const int w = tid >> 8, half = (warp >> 2) & 1;  // softmax warps: row tile, half of the keys
+    const int R = row0 + w * 128 + (tid & 127);      // this thread's packed row
     int nr = 0;
-    if (live) {
+    if (tid < 2 * kTcRows && R < n_packed) {
         nr = a.vis ? min(max(a.vis[sq.r0 + R / rep], 0), sq.len) : sq.len;
-        atomicMax(&shared_i[1], nr);
+        if (half == 0) atomicMax(&shared_i[1], nr);
     }
     tc_fence_before();
     __syncthreads();
@@ -183,58 +191,73 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int n_tiles = (kend + kTcKeys - 1) / kTcKeys;
     const int t0 = (int)((long long)n_tiles * split / parts.splits), nt = (int)((long long)n_tiles * (split + 1) / parts.splits) - t0;
 
-    if (warp < 8) {
-        setmaxnreg_inc<184>();
-        const int w = warp >> 2;
+    if (warp < 16) {
         if (w == 0 || two) {
-            // ── queries: the warp's 32 rows as f16, scaled by a power of two ──
+            const int pair = 1 + w * 4 + (warp & 3);  // barrier of the two warps that share 32 rows
+            // ── queries: half of the warp's 32 rows as f16, scaled by a power of two ──
             constexpr int LPR = HD / 8, RPI = 32 / LPR;  // lanes of a row (16 bytes each), rows of one load
             const uint32_t tm_s = tmem + w * 128 + ((uint32_t)(warp & 3) << 21), tm_o = tmem + 256 + w * 128 + ((uint32_t)(warp & 3) << 21);
-            const int wrow = row0 + warp * 32;  // the warp's first packed row
-            uint8_t *stage = sm + L::q_off + w * L::q + (warp & 3) * 32 * (HD * 2);
+            const int wrow = row0 + w * 128 + (warp & 3) * 32;  // the warp's first packed row
+            float *crow = reinterpret_cast<float *>(sm + L::crow_off) + w * 128 + (warp & 3) * 32;
             float cr = fabsf(a.scale) * kLog2e;
             if (nt > 0) {  // (without keys the output goes through this memory right away)
-                uint4 raw[LPR];
-                const int ch = lane % LPR, sub = lane / LPR;
+                uint4 raw[LPR / 2];
+                const int ch = lane % LPR, r0 = half * 16 + lane / LPR;
+                const T *from[LPR / 2];
 #pragma unroll
-                for (int i = 0; i < LPR; i++) {
-                    const int r = wrow + i * RPI + sub;
-                    raw[i] = make_uint4(0, 0, 0, 0);
-                    if (r < n_packed) {
-                        const T *q = reinterpret_cast<const T *>(a.q) + (sq.r0 + r / rep) * a.q_tok + (kvh * rep + r % rep) * a.q_head + 8 * ch;
-                        if (vec) raw[i] = *reinterpret_cast<const uint4 *>(q);
-                        else
-#pragma unroll
-                            for (int e = 0; e < 8; e++) reinterpret_cast<T *>(&raw[i])[e] = q[e];
-                    }
+                for (int i = 0; i < LPR / 2; i++) {
+                    // (a row that does not exist is read as the last one: what comes of it is not stored)
+                    const int r = min(wrow + r0 + i * RPI, n_packed - 1), t = r / rep;
+                    from[i] = reinterpret_cast<const T *>(a.q) + (sq.r0 + t) * a.q_tok + (kvh * rep + r - t * rep) * a.q_head + 8 * ch;
                 }
-                float mine = 1.f;
+                if (vec) {
 #pragma unroll
-                for (int i = 0; i < LPR; i++) {
-                    float x[8], up = 1.f;
+                    for (int i = 0; i < LPR / 2; i++) raw[i] = *reinterpret_cast<const uint4 *>(from[i]);
+                } else {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = to_f32<T>(reinterpret_cast<const T *>(&raw[i])[e]);
-                    if constexpr (!std::is_same<T, __half>::value) {
-                        float mx = 0.f;
+                    for (int i = 0; i < LPR / 2; i++)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
+                        for (int e = 0; e < 8; e++) reinterpret_cast<T *>(&raw[i])[e] = from[i][e];
+                }
+                float up[LPR / 2];
 #pragma unroll
-                        for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        const int e = (int)(__float_as_uint(mx) >> 23) - 127;
-                        if (mx > 0.f && mx < INFINITY) up = exp2i(min(max(-e, -126), 60));
-                        const float got = __shfl_sync(0xffffffffu, up, (lane % RPI) * LPR);  // of row i * RPI + lane % RPI
-                        if (lane / RPI == i) mine = got;
+                for (int i = 0; i < LPR / 2; i++) up[i] = 1.f;
+                if constexpr (!std::is_same<T, __half>::value) {
+                    float mx[LPR / 2];
+#pragma unroll
+                    for (int i = 0; i < LPR / 2; i++) {
+                        mx[i] = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) mx[i] = fmaxf(mx[i], fabsf(to_f32<T>(reinterpret_cast<const T *>(&raw[i])[e])));
                     }
-                    up = a.scale < 0.f ? -up : up;  // a negative scale turns q's sign: the factors of the scores stay positive
+#pragma unroll
+                    for (int o = 1; o < LPR; o <<= 1)
+#pragma unroll
+                        for (int i = 0; i < LPR / 2; i++) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+#pragma unroll
+                    for (int i = 0; i < LPR / 2; i++) {
+                        const int e = (int)(__float_as_uint(mx[i]) >> 23) - 127;
+                        up[i] = mx[i] > 0.f && mx[i] < INFINITY ? exp2i(min(max(-e, -126), 60)) : 1.f;
+                    }
+                    if (ch == 0)
+#pragma unroll
+                        for (int i = 0; i < LPR / 2; i++) crow[r0 + i * RPI] = 1.f / up[i];
+                }
+#pragma unroll
+                for (int i = 0; i < LPR / 2; i++) {
+                    float x[8];
+                    const int rt = (warp & 3) * 32 + r0 + i * RPI;
+                    const float f = a.scale < 0.f ? -up[i] : up[i];  // a negative scale turns q's sign: the scores' factors stay positive
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = to_f32<T>(reinterpret_cast<const T *>(&raw[i])[e]) * f;
                     uint4 u;
-                    u.x = pack_f16(x[0] * up, x[1] * up); u.y = pack_f16(x[2] * up, x[3] * up);
-                    u.z = pack_f16(x[4] * up, x[5] * up); u.w = pack_f16(x[6] * up, x[7] * up);
-                    const int r = (warp & 3) * 32 + i * RPI + sub;
-                    *reinterpret_cast<uint4 *>(sm + L::q_off + w * L::q + (ch / 8) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = u;
+                    u.x = pack_f16(x[0], x[1]); u.y = pack_f16(x[2], x[3]);
+                    u.z = pack_f16(x[4], x[5]); u.w = pack_f16(x[6], x[7]);
+                    *reinterpret_cast<uint4 *>(sm + L::q_off + w * L::q + (ch / 8) * 16384 + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4)) = u;
                 }
-                cr *= 1.f / mine;
                 fence_proxy_async_smem();
-                __syncwarp();
+                named_bar_sync(pair, 64);
+                if constexpr (!std::is_same<T, __half>::value) cr *= crow[lane];
                 if (lane == 0) mbar_arrive(bar_q);
             }
             // ── key tiles ──
@@ -242,141 +265,160 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int j = 0; j < nt; j++) {
                 if (!attn_wait(&bar_s[w], j & 1, abort_flag)) break;
                 if (wrow >= n_packed) {  // no row of this warp exists: whatever its lanes of P hold, no one reads what comes of it
-                    if (lane == 0) {
-                        mbar_arrive(&bar_pa[w]);
-                        mbar_arrive(&bar_pb[w]);
-                    }
+                    if (lane == 0) mbar_arrive(half ? &bar_pb[w] : &bar_pa[w]);
                     continue;
                 }
                 tc_fence_after();
-                float x[128];
+                const float4 *g = sc + (j & 3) * 8 + 4 * half;
+                const int left = nr - (t0 + j) * kTcKeys - 64 * half;  // keys of this half that the row sees
+                const bool cut = __any_sync(0xffffffffu, left < 64 || g[0].w != 0.f);  // (keys of a bad page: rare)
+                // 32 scores at a time: all 64 in registers would spill, and the memory behind a spill is L2 here
+                float x[32];
+                auto fetch = [&](int q) {
+                    tmem_ld32(tm_s + 64 * half + 32 * q, x);
+                    tmem_ld_wait32(x);
+                    if (cut) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) tmem_ld32(tm_s + 32 * i, x + 32 * i);
+                        for (int p = 0; p < 2; p++) {
+                            const bool none = g[2 * q + p].y == -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; i++) tmem_ld_wait32(x + 32 * i);
-                const float4 *g = sc + (j & 3) * 8;
-                const int left = nr - (t0 + j) * kTcKeys;  // keys of the tile this row sees
-                const bool holes = g[0].w != 0.f;
-                // rows that see only a part of the tile, keys of a bad page: rare
-                if (__any_sync(0xffffffffu, left < kTcKeys || holes)) {
-#pragma unroll
-                    for (int p = 0; p < 8; p++) {
-                        const bool none = g[p].y == -INFINITY;
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            if (16 * p + e >= left || none) x[16 * p + e] = -INFINITY;
+                            for (int e = 0; e < 16; e++)
+                                if (32 * q + 16 * p + e >= left || none) x[16 * p + e] = -INFINITY;
+                        }
                     }
-                }
-                // the largest t = s fk + lv of the tile: by runs, whose factor is not negative
-                float mx = -INFINITY;
-#pragma unroll
-                for (int p = 0; p < 8; p += 2) {
-                    const float4 f = g[p], f1 = g[p + 1];
+                };
+                // the largest t = s fk + lv: by runs, whose factor is not negative
+                auto top = [&](int q) {
+                    const float4 f = g[2 * q], f1 = g[2 * q + 1];
                     float m[4];
 #pragma unroll
                     for (int h = 0; h < 4; h++) {
-                        const float *y = x + 16 * p + 8 * h;
+                        const float *y = x + 8 * h;
                         m[h] = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), fmaxf(y[6], y[7]));
                     }
-                    mx = max3(mx, fmaf(fmaxf(m[0], m[1]), fmaxf(cr * f.x, kMinFactor), f.y), fmaf(fmaxf(m[2], m[3]), fmaxf(cr * f1.x, kMinFactor), f1.y));
-                }
-                mx -= kTcOff;
-                // follow the maximum only by jumps: most tiles leave O as it is
-                if (__any_sync(0xffffffffu, mx > M + kTcSlack || (M == -INFINITY && mx > M))) {
+                    return fmaxf(fmaf(fmaxf(m[0], m[1]), fmaxf(cr * f.x, kMinFactor), f.y), fmaf(fmaxf(m[2], m[3]), fmaxf(cr * f1.x, kMinFactor), f1.y));
+                };
+                fetch(1);
+                float mx = top(1);
+                fetch(0);
+                mx = fmaxf(mx, top(0)) - kTcOff;
+                // follow the maximum only by jumps: most tiles leave M and O as they are, and the two
+                // threads of a row need not tell each other more than that
+                if (named_bar_any(pair, 64, mx > M + kTcSlack || (M == -INFINITY && mx > M))) {
+                    if (half) crow[lane] = mx;
+                    named_bar_sync(pair, 64);
+                    if (!half) crow[lane] = mx = fmaxf(mx, crow[lane]);
+                    named_bar_sync(pair, 64);
+                    if (half) mx = crow[lane];
                     const float mn = fmaxf(M, mx), al = mn == -INFINITY ? 1.f : ex2(M - mn);
                     M = mn;
                     l *= al;
                     if (j > 0) {
 #pragma unroll
                         for (int i = 0; i < HD / 32; i++) {
-                            float o[32];
-                            tmem_ld32(tm_o + 32 * i, o);
-                            tmem_ld_wait32(o);
+                            const uint32_t at = tm_o + half * (HD / 2) + 16 * i;
+                            uint32_t u[16];
+                            tmem_ld16(at, u);
+                            tmem_ld_wait(u);
 #pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                uint32_t u[16];
-#pragma unroll
-                                for (int e = 0; e < 16; e++) u[e] = __float_as_uint(o[16 * h + e] * al);
-                                tmem_st16(tm_o + 32 * i + 16 * h, u);
-                            }
+                            for (int e = 0; e < 16; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * al);
+                            tmem_st16(at, u);
                         }
                     }
                 }
                 const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll
-                for (int p = 0; p < 8; p += 2) {
+                for (int q = 0; q < 2; q++) {
+                    if (q == 1) fetch(1);
                     uint32_t u[16];
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const float4 f = g[p + h];
+                        const float4 f = g[2 * q + h];
                         const float fk = fmaxf(cr * f.x, kMinFactor), add = f.y - base;
                         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            const float2 y = fma2(make_float2(x[16 * (p + h) + e], x[16 * (p + h) + e + 1]), make_float2(fk, fk), make_float2(add, add));
+                            const float2 y = fma2(make_float2(x[16 * h + e], x[16 * h + e + 1]), make_float2(fk, fk), make_float2(add, add));
                             const float2 pr = make_float2(ex2(y.x), ex2(y.y));
                             sum = add2(sum, pr);
                             u[8 * h + e / 2] = pack_f16(pr.x, pr.y);
                         }
                         l = fmaf(sum.x + sum.y, f.z, l);
                     }
-                    tmem_st16(tm_s + 8 * p, u);
-                    if (p == 2 || p == 6) {  // each half of the tile's keys on its own: its P V starts under the other's exponentials
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(p == 2 ? &bar_pa[w] : &bar_pb[w]);
-                    }
+                    tmem_st16(tm_s + 64 * half + 16 * q, u);  // (below the scores that are still to be fetched)
                 }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(half ? &bar_pb[w] : &bar_pa[w]);
             }
             // ── output ──
             bool ok = true;
             if (nt > 0) ok = attn_wait(&bar_o[w], 0, abort_flag);
             tc_fence_after();
             if (!ok && status) atomicOr(status, DFB_STAT_TIMEOUT);
+            // (the query tile is free: its last reader was the last score MMA)
+            float *lx = reinterpret_cast<float *>(sm + L::q_off + w * L::q) + (warp & 3) * 64;
+            if (nt == 0) named_bar_sync(pair, 64);
+            lx[half * 32 + lane] = l;
+            named_bar_sync(pair, 64);
+            l += lx[(1 - half) * 32 + lane];
             const float inv = l > 0.f ? 1.f / l : 0.f, lw = l > 0.f ? M + log2f(l) : -INFINITY;
-            // through the warp's part of the query tile (its last reader was the last score MMA), so that
-            // rows leave as whole 16-byte columns of consecutive lanes
             const int own = wrow + lane;  // this thread's packed row
-            if (own < n_packed) {
+            if (half == 0 && own < n_packed) {
                 const size_t row = (size_t)(sq.r0 + own / rep) * a.n_q + kvh * rep + own % rep;
                 if (parts.o) parts.w[(size_t)split * a.n_rows * a.n_q + row] = lw;
                 else if (a.lse) a.lse[row] = lw * kLn2;
             }
+            named_bar_sync(9 + w, 256);  // every lx is read
+            // through shared memory, so that rows leave as whole 16-byte columns of consecutive lanes: each
+            // warp has half of the dimensions of its rows, in passes of HD bytes
+            uint8_t *stage = sm + L::q_off + w * L::q + ((warp & 3) * 2 + half) * 32 * HD;
             auto put = [&](auto zero, int pass) {  // zero's type: of the stored elements
                 using E = decltype(zero);
-                constexpr int PER = 16 / sizeof(E), N = HD * 2 / sizeof(E);  // elements of a column, of a pass
+                constexpr int PER = 16 / sizeof(E), N = HD / sizeof(E), CPR = HD / 16;  // elements of a column and of a pass, columns of a row
+                const int d0 = half * (HD / 2) + pass * N;
 #pragma unroll
-                for (int i = 0; i < N / 32; i++) {
-                    float o[32];
+                for (int i = 0; i < N / 16; i++) {
+                    float o[16] = {};
                     if (nt > 0) {
-                        tmem_ld32(tm_o + pass * N + 32 * i, o);
-                        tmem_ld_wait32(o);
+                        uint32_t u[16];
+                        tmem_ld16(tm_o + d0 + 16 * i, u);
+                        tmem_ld_wait(u);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = __uint_as_float(u[e]);
                     }
 #pragma unroll
-                    for (int h = 0; h < 32 / PER; h++) {
+                    for (int h = 0; h < 16 / PER; h++) {
                         E t[PER];
 #pragma unroll
                         for (int e = 0; e < PER; e++) t[e] = from_f32<E>(l > 0.f ? o[PER * h + e] * inv : 0.f);
-                        const int ch = i * (32 / PER) + h;
-                        *reinterpret_cast<uint4 *>(stage + lane * (HD * 2) + ((ch ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4 *>(t);
+                        const int ch = i * (16 / PER) + h;
+                        *reinterpret_cast<uint4 *>(stage + lane * HD + ((ch ^ (lane & (CPR - 1))) << 4)) = *reinterpret_cast<const uint4 *>(t);
                     }
                 }
                 __syncwarp();
-                const int ch = lane % LPR;
+                const int ch = lane % CPR;
+                auto dst = [&](int r) {  // of packed row r
+                    const int t = r / rep, tok = sq.r0 + t, head = kvh * rep + r - t * rep;
+                    E *d = sizeof(E) == 4 ? reinterpret_cast<E *>(parts.o) + ((size_t)split * a.n_rows * a.n_q + (size_t)tok * a.n_q + head) * HD
+                                          : reinterpret_cast<E *>(a.out) + tok * a.out_tok + head * a.out_head;
+                    return d + d0 + ch * PER;
+                };
+                uint4 u[CPR];
 #pragma unroll
-                for (int i = 0; i < LPR; i++) {
-                    const int r = i * RPI + lane / LPR, R = wrow + r;
-                    const uint4 u = *reinterpret_cast<const uint4 *>(stage + r * (HD * 2) + ((ch ^ (r & 7)) << 4));
-                    if (R >= n_packed) continue;
-                    const int tok = sq.r0 + R / rep, head = kvh * rep + R % rep;
-                    E *dst = sizeof(E) == 4 ? reinterpret_cast<E *>(parts.o) + ((size_t)split * a.n_rows * a.n_q + (size_t)tok * a.n_q + head) * HD
-                                            : reinterpret_cast<E *>(a.out) + tok * a.out_tok + head * a.out_head;
-                    dst += pass * N + ch * PER;
-                    if (sizeof(E) == 4 || vec) *reinterpret_cast<uint4 *>(dst) = u;
+                for (int i = 0; i < CPR; i++) {
+                    const int r = i * (32 / CPR) + lane / CPR;
+                    u[i] = *reinterpret_cast<const uint4 *>(stage + r * HD + ((ch ^ (r & (CPR - 1))) << 4));
+                }
+#pragma unroll
+                for (int i = 0; i < CPR; i++) {
+                    const int r = wrow + i * (32 / CPR) + lane / CPR;
+                    if (r >= n_packed) break;
+                    if (sizeof(E) == 4 || vec) *reinterpret_cast<uint4 *>(dst(r)) = u[i];
                     else
 #pragma unroll
-                        for (int e = 0; e < PER; e++) dst[e] = reinterpret_cast<const E *>(&u)[e];
+                        for (int e = 0; e < PER; e++) dst(r)[e] = reinterpret_cast<const E *>(&u[i])[e];
                 }
                 __syncwarp();
             };
@@ -391,10 +433,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_before();
         }
     } else {
-        setmaxnreg_dec<72>();
-        if (warp < 12) {
+        if (warp < 20) {
             // ── converters ──
-            const int cw = warp - 8;
+            const int cw = warp - 16;
             for (int n = 0; n < 2 * nt; n++) {
                 const int rs = n % kTcRaw, cs = n % kTcSlots, j = n >> 1;
                 if (!attn_wait(&raw_full[rs], (n / kTcRaw) & 1, abort_flag)) break;
@@ -441,7 +482,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&conv_full[cs]);
             }
-        } else if (warp == 12) {
+        } else if (warp == 20) {
             // ── MMA issuer ──
             if (lane == 0 && nt > 0) {
                 const uint32_t id_s = idesc_f16(128, kTcKeys), id_o = idesc_f16(128, HD) | (1u << 16);  // V is MN-major
@@ -460,7 +501,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int i = 0; i < kTcKeys / 32; i++) {
                         const int k = half * (kTcKeys / 32) + i;
-                        mma1_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + 8 * k, db + (2048 >> 4) * k, id_o, add || i > 0);
+                        mma1_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + 64 * half + 8 * i, db + (2048 >> 4) * k, id_o, add || i > 0);
                     }
                 };
                 auto ready = [&](uint64_t *b, int ph) {
@@ -503,7 +544,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
             }
             __syncwarp();
-        } else if (warp == 13) {
+        } else if (warp == 21) {
             // ── loader ──
             const int box = min(c.page, kKeyTile), nb = kTcKeys / box;
             int pid = 0, issued = 0;
@@ -523,7 +564,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     ks = vs = 1.f;
                     if (pid >= 0) {
                         ks = c.k_scale[(size_t)pid * c.n_kv + kvh];
-                        vs = fmaxf(c.v_scale[(size_t)pid * c.n_kv + kvh], 5.421010862427522e-20f);
+                        vs = c.v_scale[(size_t)pid * c.n_kv + kvh];  // (first used after the tile's copies are under way)
                     }
                 }
                 if (n >= kTcRaw && !attn_wait(&raw_empty[rs], (n / kTcRaw - 1) & 1, abort_flag)) break;
@@ -541,7 +582,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     // (the entry's last readers, the softmax of tile j - 4, ended before K of tile j - 1 was converted)
                     const int src = b0 + (lane & 7) * 16 / box;
                     const int gp = __shfl_sync(0xffffffffu, pid, src);
-                    const float gk = __shfl_sync(0xffffffffu, ks, src), gv = __shfl_sync(0xffffffffu, vs, src);
+                    const float gk = __shfl_sync(0xffffffffu, ks, src), gv = fmaxf(__shfl_sync(0xffffffffu, vs, src), 5.421010862427522e-20f);
                     const bool holes = __any_sync(0xffffffffu, gp < 0);
                     if (lane < 8) sc[(j & 3) * 8 + lane] = make_float4(gk, gp < 0 ? -INFINITY : log2f(gv), 1.f / gv, holes ? 1.f : 0.f);
                 }
@@ -554,7 +595,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
     }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc_fence_after();
         tmem_dealloc1(tmem, 512);
     }
