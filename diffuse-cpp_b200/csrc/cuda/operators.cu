@@ -165,7 +165,7 @@ int attn_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, 
 
 template <typename T, int HD>
 int attn_tc_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, const AttnParts &parts, const CUtensorMap &tk,
-                   const CUtensorMap &tv, bool vec, int dev, int32_t *status, cudaStream_t st) {
+                   const CUtensorMap &tv, bool vec, int dev, int n_sm, int32_t *status, cudaStream_t st) {
     const auto kern = kv_attn_tc_kernel<T, HD>;
     constexpr int smem = TcSmem<HD>::bytes;
     static_assert(smem <= 232448, "shared memory of one CTA");
@@ -174,13 +174,18 @@ int attn_tc_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &
         CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         attr_set[dev] = true;
     }
-    kern<<<dim3(p.tiles * p.splits, c.n_kv, c.n_seq), kTcThreads, smem, st>>>(c, a, tk, tv, parts, vec, status);
+    const int64_t items = (int64_t)p.tiles * p.splits * c.n_kv * c.n_seq;
+    if (items > INT32_MAX / 2) return set_err(DFB_ERR_UNSUPPORTED, "%lld work items", (long long)items);
+    const TcGrid grid{p.tiles, (int)items};
+    // 16-bit elements: the widest store that every row's start allows
+    const int out_align = aligned(a.out, 32) && a.out_tok % 16 == 0 && a.out_head % 16 == 0 ? 32 : vec_ok(a.out, a.type, a.out_tok, a.out_head) ? 16 : 2;
+    kern<<<(unsigned)std::min<int64_t>(items, n_sm), kTcThreads, smem, st>>>(c, a, tk, tv, parts, grid, vec, out_align, status);
     CK(cudaGetLastError());
     return DFB_OK;
 }
 
 template <typename T, int HD>
-int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float *ws, int dev, int32_t *status, cudaStream_t st) {
+int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float *ws, int dev, int n_sm, int32_t *status, cudaStream_t st) {
     CUtensorMap tk, tv;
     RET(code_map(&tk, c.k, c));
     RET(code_map(&tv, c.v, c));
@@ -195,7 +200,7 @@ int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float
         case 16: RET((attn_launch<T, HD, 1, 4>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
         case 32: RET((attn_launch<T, HD, 2, 4>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
         case 64: RET((attn_launch<T, HD, 4, 2>(c, a, p, parts, tk, tv, vec, dev, status, st))); break;
-        default: RET((attn_tc_launch<T, HD>(c, a, p, parts, tk, tv, vec, dev, status, st)));
+        default: RET((attn_tc_launch<T, HD>(c, a, p, parts, tk, tv, vec, dev, n_sm, status, st)));
     }
     if (p.splits > 1) {
         const int64_t per_seq = (int64_t)a.max_rows * a.n_q;
@@ -282,7 +287,7 @@ extern "C" int dfb_kv_attention(const dfb_kv_cache *c, const dfb_kv_attn *a, voi
     float *ws = static_cast<float *>(workspace);
     auto go = [&](auto t) {
         using T = decltype(t);
-        return c->head_dim == 64 ? attn_t<T, 64>(*c, *a, p, ws, g.device(), status, st) : attn_t<T, 128>(*c, *a, p, ws, g.device(), status, st);
+        return c->head_dim == 64 ? attn_t<T, 64>(*c, *a, p, ws, g.device(), n_sm, status, st) : attn_t<T, 128>(*c, *a, p, ws, g.device(), n_sm, status, st);
     };
     return a->type == T_F16 ? go(__half()) : go(__nv_bfloat16());
 }
