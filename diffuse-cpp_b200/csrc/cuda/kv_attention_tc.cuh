@@ -1,14 +1,17 @@
 // Attention over the paged 8-bit cache for many query rows: tcgen05 MMAs on tiles of 2 x 128 packed
 // rows x 128 keys (arithmetic: kv_attention.cuh).
 //
-// A persistent CTA per SM (14 warps) takes work items -- a sequence, KV head, tile of 256 packed rows
+// A persistent CTA per SM (24 warps) takes work items -- a sequence, KV head, tile of 256 packed rows
 // and part of the keys -- in turn:
-//   warps 0-3, 4-7  softmax of row tile 0 / 1, a thread to a row (TMEM lane): scores from TMEM, p' back
-//                   into their place as f16 (the A operand of P V), rare rescales of O, the output
-//   warps 8-11      converters: E4M3 codes -> f16 operands in shared memory, both of K and of V as
+//   warps 0-7, 8-15 softmax of row tile 0 / 1, two threads to a row (TMEM lane), 64 keys each: scores
+//                   from TMEM, p' back into their place as f16 (the A operand of P V), rare rescales
+//                   of O, the output
+//   warps 16-19     converters: E4M3 codes -> f16 operands in shared memory, both of K and of V as
 //                   rows of 64 dimensions swizzled over 128 bytes (K-major for K, MN-major for V);
 //                   an item's queries
-//   warp 12         MMA issuer, warp 13 loader (one tensor copy per run of page positions)
+//   warp 20         MMA issuer
+//   warp 21         loader (one tensor copy per run of page positions); works the items out for all
+//   warp 22         the rows of items without a key
 // MMA order: S0(0) S1(0), then for each key tile j: P0 V, S0(j+1), P1 V, S1(j+1), so one row tile's
 // softmax runs under the other's MMAs; S0(j+1) is complete only after P0 V(j), so a softmax thread
 // that has its scores may rescale its row of O without another wait.  Tile "j + 1" of an item's last
@@ -22,10 +25,19 @@ namespace dfb {
 
 constexpr int kTcKeys = 128;     // keys of one tile
 constexpr int kTcRows = 256;     // packed rows of one CTA
-constexpr int kTcThreads = 512;  // (two warps do nothing: registers are handed out to four warps at a time)
-constexpr int kTcRaw = 2;        // raw slots: 128 x HD codes of K or V
-constexpr int kTcSlots = 4;      // f16 slots, K and V of successive tiles in turn
+constexpr int kTcThreads = 768;  // 80 registers each (one warp does nothing: registers go to four warps at a time)
+// Raw slots (128 x HD codes of K or V) and f16 slots, K and V of successive tiles in turn.  Two tiles of
+// codes in flight hide memory's latency (with one, 64 x 256 x 768 took 276 us without any softmax);
+// the f16 slots hold what an MMA may read and one more.
+constexpr int kTcRaw = 4, kTcSlots = 3;
 constexpr float kTcOff = 7.f, kTcSlack = 8.f;  // p' <= 2^(off + slack) = 2^15 although the maximum is only followed by jumps
+
+// One work item with keys, as the loader describes it in shared memory; nt < 0: there are no more.
+struct TcItem {
+    int s, kvh, split, r0, len, row0, n_packed, kend, t0, nt;
+};
+constexpr int kTcItems = 4;       // entries
+constexpr int kTcItemUsers = 21;  // warps that read them
 
 template <int HD>
 struct TcSmem {
@@ -34,8 +46,9 @@ struct TcSmem {
     static constexpr int raw = kTcKeys * HD;
     static constexpr int q_off = 0, slot_off = 2 * q, raw_off = slot_off + kTcSlots * slot, sc_off = raw_off + kTcRaw * raw;
     static constexpr int bar_off = sc_off + 4 * 8 * 16;
-    static constexpr int n_bars = 2 * kTcRaw + kTcSlots + 13;
-    static constexpr int crow_off = bar_off + n_bars * 8 + 32;
+    static constexpr int n_bars = 2 * kTcRaw + kTcSlots + 13 + 2 * kTcItems;
+    static constexpr int item_off = bar_off + n_bars * 8 + 16;
+    static constexpr int crow_off = item_off + kTcItems * (int)sizeof(TcItem);
     static constexpr int bytes = 1024 + crow_off + 2 * kTcRows;
 };
 
@@ -49,15 +62,35 @@ __device__ __forceinline__ void tmem_dealloc1(uint32_t taddr, uint32_t ncols) {
 __device__ __forceinline__ void mma1_commit(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void mma1_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-                 "r"(idesc), "r"(acc)
+// D (+)= A B^T with A from shared memory / from TMEM; D, A: TMEM columns.  A kernel that takes all 512
+// columns has them from address 0 on, so they are constants here: operands that the compiler can
+// keep in uniform registers issue without a move per operand.
+template <int D, bool ADD>
+__device__ __forceinline__ void mma1_f16_ss(uint64_t a, uint64_t b, uint32_t idesc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(D), "l"(a), "l"(b),
+                 "r"(idesc), "n"((int)ADD)
                  : "memory");
 }
-__device__ __forceinline__ void mma1_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b),
-                 "r"(idesc), "r"(acc)
+template <int D, int A>
+__device__ __forceinline__ void mma1_f16_ts(uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(D), "r"(A), "l"(b),
+                 "r"(idesc), "r"((int)add)
                  : "memory");
+}
+template <int I>
+using Int = std::integral_constant<int, I>;
+// f(Int<0>), ..., f(Int<N - 1>)
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void unrolled(F &&f) {
+    if constexpr (I < N) {
+        f(Int<I>());
+        unrolled<N, I + 1>(f);
+    }
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
 }
 // 32 lanes x 32 columns: this thread's lane, columns [col, col + 32).
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
@@ -83,7 +116,29 @@ __device__ __forceinline__ void tmem_ld_wait32(float *r) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
+}
+__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(v) : "r"(taddr) : "memory");
+    return __uint_as_float(v);
+}
+// Whether any of the n threads of a named barrier passes true.
+__device__ __forceinline__ bool named_bar_any(uint32_t id, uint32_t n, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbarrier.cta.red.or.aligned.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"(n), "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
+}
 // Two f32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     uint64_t d;
@@ -100,19 +155,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // The factor of a score is kept above 0, so that a masked score of -inf stays -inf where the softmax
 // scale is 0 or the product of the scales underflows; every score times this is 0 beside an exponent.
 constexpr float kMinFactor = 1.1754944e-38f;
-// Bounded wait of one thread (the MMA issuer and single waits); see attn_wait.
-__device__ __forceinline__ bool thread_wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer();
-    while (!mbar_try_wait_sleep(bar, parity, kWaitCheckNs)) {
-        if (*abort_flag) return false;
-        if (globaltimer() - t0 > kWaitTimeoutNs) {
-            *abort_flag = 1;
-            return false;
-        }
-    }
-    return true;
-}
 // MN-major operand, rows (k) of 64 elements (128 bytes) swizzled over 128 bytes: 8-row groups 1024
 // bytes apart, 64-element blocks `block` bytes apart.
 __device__ __forceinline__ uint64_t mn128_desc(uint32_t smem_addr, uint32_t block) {
@@ -143,17 +185,10 @@ __device__ __forceinline__ void store_row32(E *p, int align, const uint32_t (&u)
         for (int e = 0; e < 32 / (int)sizeof(E); e++) p[e] = reinterpret_cast<const E *>(u)[e];
 }
 
-// One work item; every warp of the CTA works out the same.
-struct TcItem {
-    int s, kvh, split;
-    AttnSeq sq;
-    int row0, n_packed, kend, t0, nt;
-    bool two;
-};
 struct TcGrid {
     int tiles, items;  // row tiles of a sequence (at most), work items
 };
-// The idx-th item; false if it has no rows.  Called by whole warps.
+// The idx-th item; false if it has no rows.  Called by a whole warp.
 __device__ __forceinline__ bool tc_item(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnParts &parts, const TcGrid &grid, int rep, int idx,
                                         int32_t *status, TcItem &it) {
     const int per = grid.tiles * parts.splits, lane = threadIdx.x & 31;
@@ -161,16 +196,16 @@ __device__ __forceinline__ bool tc_item(const dfb_kv_cache &c, const dfb_kv_attn
     it.split = x % parts.splits;
     it.kvh = y % c.n_kv;
     it.s = y / c.n_kv;
-    it.sq = attn_seq(c, a, it.s, x == 0 && it.kvh == 0 && threadIdx.x == 0, status);
+    const AttnSeq sq = attn_seq(c, a, it.s, x == 0 && it.kvh == 0 && lane == 0, status);
+    it.r0 = sq.r0;
+    it.len = it.kend = sq.len;
     it.row0 = x / parts.splits * kTcRows;
-    it.n_packed = it.sq.n_rows * rep;
+    it.n_packed = sq.n_rows * rep;
     if (it.row0 >= it.n_packed) return false;
-    it.two = it.row0 + 128 < it.n_packed;
-    it.kend = it.sq.len;
     if (a.vis) {  // the most keys any of the item's tokens sees
         const int last = (min(it.row0 + kTcRows, it.n_packed) - 1) / rep;
         int n = 0;
-        for (int t = it.row0 / rep + lane; t <= last; t += 32) n = max(n, a.vis[it.sq.r0 + t]);
+        for (int t = it.row0 / rep + lane; t <= last; t += 32) n = max(n, a.vis[it.r0 + t]);
         it.kend = min(it.kend, max(0, __reduce_max_sync(0xffffffffu, n)));
     }
     const int n = (it.kend + kTcKeys - 1) / kTcKeys;
@@ -189,7 +224,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float4 *sc = reinterpret_cast<float4 *>(sm + L::sc_off);  // [tile & 3][8 runs of 16 keys] ks, log2 vs, 1 / vs, any absent
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + L::bar_off);
     uint64_t *raw_full = bars, *raw_empty = raw_full + kTcRaw, *conv_full = raw_empty + kTcRaw, *freed = conv_full + kTcSlots;
-    uint64_t *bar_s = freed + 2, *bar_pa = bar_s + 2, *bar_pb = bar_pa + 2, *bar_o = bar_pb + 2, *bar_q = bar_o + 2, *bar_drain = bar_q + 2;
+    uint64_t *bar_s = freed + 2, *bar_pa = bar_s + 2, *bar_pb = bar_pa + 2, *bar_o = bar_pb + 2, *bar_q = bar_o + 2, *item_full = bar_q + 2,
+             *item_empty = item_full + kTcItems, *bar_drain = item_empty + kTcItems;
     int *shared_i = reinterpret_cast<int *>(bars + L::n_bars);  // abort flag, TMEM address
     volatile int *abort_flag = shared_i;
 
@@ -210,273 +246,281 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar_o[i], 1);
             mbar_init(&bar_q[i], 4);
         }
+        for (int i = 0; i < kTcItems; i++) {
+            mbar_init(&item_full[i], 1);
+            mbar_init(&item_empty[i], kTcItemUsers);
+        }
         mbar_init(bar_drain, 1);
         fence_barrier_init();
     }
-    if (warp == 12) tmem_alloc1(reinterpret_cast<uint32_t *>(&shared_i[1]), 512);
+    if (warp == 20) tmem_alloc1(reinterpret_cast<uint32_t *>(&shared_i[1]), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = (uint32_t)shared_i[1];
-    TcItem it;
+    const uint32_t tmem = 0;  // (all 512 columns are this CTA's)
+    const volatile TcItem *items = reinterpret_cast<const volatile TcItem *>(sm + L::item_off);
 
-    if (warp < 8) {
+    if (warp < 16) {
         // ── softmax ──
-        const int w = warp >> 2;  // row tile
-        const uint32_t tm_s = tmem + w * 128 + ((uint32_t)(warp & 3) << 21), tm_o = tm_s + 256;
-        // exponents of the queries' scales, by the parity of the item: one is written while the other may still be read
-        const int8_t *crow = reinterpret_cast<const int8_t *>(sm + L::crow_off) + w * 128 + (warp & 3) * 32 + lane;
-        int odd = 0;
-        uint32_t ph_s = 0, ph_o = 0;
+        const int w = warp >> 3, half = (warp >> 2) & 1;  // row tile, half of its keys
+        const int pair = 1 + w * 4 + (warp & 3);          // barrier of the two warps that share 32 rows
+        const uint32_t tm_s = tmem + w * 128 + 64 * half + ((uint32_t)(warp & 3) << 21);  // this half's scores; 64 ^: the other's
+        const uint32_t tm_o = tmem + 256 + w * 128 + half * (HD / 2) + ((uint32_t)(warp & 3) << 21);  // this half of the dimensions
+        const int in_tile = w * 128 + (warp & 3) * 32;  // the warp's first row in the item
+        uint32_t ph_s = 0, ph_o = 0, odd = 0;
         int g = 0;  // key tiles of the CTA so far
         bool ok = true;
-        for (int idx = blockIdx.x; ok && idx < grid.items; idx += gridDim.x) {
-            if (!tc_item(c, a, parts, grid, rep, idx, status, it)) continue;
-            odd ^= it.nt > 0;
-            if (w == 1 && !it.two) {
-                g += it.nt;
-                continue;
-            }
-            const int wrow = it.row0 + w * 128 + (warp & 3) * 32;  // the warp's first packed row
-            const bool dead = wrow >= it.n_packed;  // no row of this warp exists: whatever its lanes of P hold, no one reads what comes of it
-            const int R = min(wrow + lane, it.n_packed - 1), tok = it.sq.r0 + R / rep, head = it.kvh * rep + R % rep;
-            int left = (a.vis ? min(max(a.vis[tok], 0), it.sq.len) : it.sq.len) - it.t0 * kTcKeys;  // keys of the tile that the row sees
-            float cr = fabsf(a.scale) * kLog2e, M = -INFINITY, l = 0.f;
-            for (int j = 0; j < it.nt; j++, g++, left -= kTcKeys) {
-                if (!(ok = attn_wait(&bar_s[w], ph_s, abort_flag))) break;
-                ph_s ^= 1;
-                if (dead) {
-                    if (lane == 0) {
-                        mbar_arrive(&bar_pa[w]);
-                        mbar_arrive(&bar_pb[w]);
-                    }
-                    continue;
+        for (int k = 0;; k++) {
+            const volatile TcItem *it = items + (k & (kTcItems - 1));
+            if (!(ok = attn_wait(&item_full[k & (kTcItems - 1)], (k / kTcItems) & 1, abort_flag))) break;
+            const int nt = it->nt;
+            if (nt < 0) break;
+            odd ^= 1;
+            if (w == 1 && it->row0 + 128 >= it->n_packed) {  // no row tile 1
+                g += nt;
+            } else {
+                const bool dead = it->row0 + in_tile >= it->n_packed;  // no row of this warp exists: no one reads what comes of its lanes
+                float cr = fabsf(a.scale) * kLog2e, M = -INFINITY, l = 0.f;
+                int left;  // keys of this half of the tile that the row sees
+                {
+                    const int len = it->len;
+                    left = len;
+                    if (a.vis) left = min(max(a.vis[it->r0 + min(it->row0 + in_tile + lane, it->n_packed - 1) / rep], 0), len);
+                    left -= it->t0 * kTcKeys + 64 * half;
                 }
-                tc_fence_after();
-                if (!std::is_same<T, __half>::value && j == 0) cr *= exp2i(crow[odd * kTcRows]);
-                const float4 *gs = sc + (g & 3) * 8;
-                const bool cut = __any_sync(0xffffffffu, left < kTcKeys || gs[0].w != 0.f);  // (keys of a bad page: rare)
-                // Scores come 32 at a time, twice (for the maximum, for the exponentials), the next 32 under way:
-                // a loop that the instruction cache next to the scheduler holds beside the other roles' loops,
-                // and no spills (the memory behind a spill is L2: 227 KB of shared memory are in use).
-                float xa[32], xb[32];
-                auto mask = [&](float (&x)[32], int q) {
-                    if (cut)
+                for (int j = 0; j < nt; j++, g++, left -= kTcKeys) {
+                    if (!(ok = attn_wait(&bar_s[w], ph_s, abort_flag))) break;
+                    ph_s ^= 1;
+                    if (dead) {
+                        if (lane == 0) mbar_arrive(half ? &bar_pb[w] : &bar_pa[w]);
+                        continue;
+                    }
+                    tc_fence_after();
+                    // exponents of the queries' scales, by the parity of the item: one is written while the other may still be read
+                    if (!std::is_same<T, __half>::value && j == 0)
+                        cr *= exp2i(reinterpret_cast<const int8_t *>(sm + L::crow_off)[odd * kTcRows + in_tile + lane]);
+                    const float4 *gs = sc + (g & 3) * 8 + 4 * half;
+                    const bool cut = __any_sync(0xffffffffu, left < 64 || gs[0].w != 0.f);  // (keys of a bad page: rare)
+                    // 32 scores at a time: 64 would spill, and the memory behind a spill is L2 (227 KB of shared
+                    // memory are in use)
+                    float x[32];
+                    auto fetch = [&](int q) {
+                        tmem_ld32(tm_s + 32 * q, x);
+                        tmem_ld_wait32(x);
+                        if (cut)
+#pragma unroll
+                            for (int p = 0; p < 2; p++) {
+                                const int n = gs[2 * q + p].y == -INFINITY ? 0 : left - 32 * q - 16 * p;
+#pragma unroll
+                                for (int e = 0; e < 16; e++)
+                                    if (e >= n) x[16 * p + e] = -INFINITY;
+                            }
+                    };
+                    // the largest t = s fk + lv: by runs, whose factor is not negative
+                    auto top = [&](int q, float mx) {
 #pragma unroll
                         for (int p = 0; p < 2; p++) {
-                            const int n = gs[2 * q + p].y == -INFINITY ? 0 : left - 32 * q - 16 * p;
-#pragma unroll
-                            for (int e = 0; e < 16; e++)
-                                if (e >= n) x[16 * p + e] = -INFINITY;
+                            const float4 f = gs[2 * q + p];
+                            const float *y = x + 16 * p;
+                            const float m0 = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), max3(y[6], y[7], y[8]));
+                            const float m1 = max3(max3(y[9], y[10], y[11]), max3(y[12], y[13], y[14]), y[15]);
+                            mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fmaxf(cr * f.x, kMinFactor), f.y));
                         }
-                };
-                float mx = -INFINITY;
-                // the largest t = s fk + lv: by runs, whose factor is not negative
-                auto top = [&](const float (&x)[32], int q) {
-#pragma unroll
-                    for (int p = 0; p < 2; p++) {
-                        const float4 f = gs[2 * q + p];
-                        const float *y = x + 16 * p;
-                        const float m0 = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], y[5]), fmaxf(y[6], y[7]));
-                        const float m1 = max3(max3(y[8], y[9], y[10]), max3(y[11], y[12], y[13]), fmaxf(y[14], y[15]));
-                        mx = fmaxf(mx, fmaf(fmaxf(m0, m1), fmaxf(cr * f.x, kMinFactor), f.y));
-                    }
-                };
-                tmem_ld32(tm_s, xa);
+                        return mx;
+                    };
+                    fetch(1);
+                    float mx = top(1, -INFINITY);
+                    fetch(0);
+                    mx = top(0, mx) - kTcOff;
+                    // follow the maximum only by jumps: most tiles leave M and O as they are, and the two
+                    // threads of a row need not tell each other more than that
+                    if (named_bar_any(pair, 64, mx > M + kTcSlack || (M == -INFINITY && mx > M))) {
+                        tmem_st1(tm_s + 16, mx);  // (a column whose score both threads' registers hold)
+                        tmem_st_wait();
+                        tc_fence_before();
+                        named_bar_sync(pair, 64);
+                        tc_fence_after();
+                        mx = fmaxf(mx, tmem_ld1((tm_s ^ 64) + 16));
+                        tc_fence_before();
+                        named_bar_sync(pair, 64);  // both are read before P is written there
+                        tc_fence_after();
+                        const float mn = fmaxf(M, mx), al = mn == -INFINITY ? 1.f : ex2(M - mn);
+                        M = mn;
+                        l *= al;
+                        if (j > 0) {
 #pragma unroll 1
-                for (int q = 0; q < 4; q += 2) {
-                    tmem_ld_wait32(xa);
-                    tmem_ld32(tm_s + 32 * q + 32, xb);
-                    mask(xa, q);
-                    top(xa, q);
-                    tmem_ld_wait32(xb);
-                    tmem_ld32(tm_s + ((32 * q + 64) & 127), xa);  // (in the end the first ones again)
-                    mask(xb, q + 1);
-                    top(xb, q + 1);
-                }
-                mx -= kTcOff;
-                // follow the maximum only by jumps: most tiles leave M and O as they are
-                if (__any_sync(0xffffffffu, mx > M + kTcSlack || (M == -INFINITY && mx > M))) {
-                    const float mn = fmaxf(M, mx), al = mn == -INFINITY ? 1.f : ex2(M - mn);
-                    M = mn;
-                    l *= al;
-                    if (j > 0) {
+                            for (int i = 0; i < HD / 32; i++) {
+                                uint32_t u[16];
+                                tmem_ld16(tm_o + 16 * i, u);
+                                tmem_ld_wait(u);
 #pragma unroll
-                        for (int i = 0; i < HD / 16; i++) {
-                            uint32_t u[16];
-                            tmem_ld16(tm_o + 16 * i, u);
-                            tmem_ld_wait(u);
-#pragma unroll
-                            for (int e = 0; e < 16; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * al);
-                            tmem_st16(tm_o + 16 * i, u);
+                                for (int e = 0; e < 16; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * al);
+                                tmem_st16(tm_o + 16 * i, u);
+                            }
                         }
                     }
-                }
-                const float base = M == -INFINITY ? 0.f : M;
-                auto exps = [&](const float (&x)[32], int q) {
-                    uint32_t u[16];
-#pragma unroll
-                    for (int p = 0; p < 2; p++) {
-                        const float4 f = gs[2 * q + p];
-                        const float fk = fmaxf(cr * f.x, kMinFactor), add = f.y - base;
-                        float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const float2 y = fma2(make_float2(x[16 * p + e], x[16 * p + e + 1]), make_float2(fk, fk), make_float2(add, add));
-                            const float2 pr = make_float2(ex2(y.x), ex2(y.y));
-                            sum = add2(sum, pr);
-                            u[8 * p + e / 2] = pack_f16(pr.x, pr.y);
-                        }
-                        l = fmaf(sum.x + sum.y, f.z, l);
-                    }
-                    tmem_st16(tm_s + 16 * q, u);  // (below the scores that are still to come)
-                };
+                    const float base = M == -INFINITY ? 0.f : M;
 #pragma unroll 1
-                for (int q = 0; q < 4; q += 2) {
-                    tmem_ld_wait32(xa);
-                    tmem_ld32(tm_s + 32 * q + 32, xb);
-                    mask(xa, q);
-                    exps(xa, q);
-                    tmem_ld_wait32(xb);
-                    if (q == 0) tmem_ld32(tm_s + 64, xa);
-                    mask(xb, q + 1);
-                    exps(xb, q + 1);
-                    // each half of the tile's keys on its own: its P V starts under the other's exponentials
+                    for (int q = 0; q < 2; q++) {
+                        if (q) fetch(1);
+                        uint32_t u[16];
+#pragma unroll
+                        for (int p = 0; p < 2; p++) {
+                            const float4 f = gs[2 * q + p];
+                            const float fk = fmaxf(cr * f.x, kMinFactor), add = f.y - base;
+                            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const float2 y = fma2(make_float2(x[16 * p + e], x[16 * p + e + 1]), make_float2(fk, fk), make_float2(add, add));
+                                const float2 pr = make_float2(ex2(y.x), ex2(y.y));
+                                sum = add2(sum, pr);
+                                u[8 * p + e / 2] = pack_f16(pr.x, pr.y);
+                            }
+                            l = fmaf(sum.x + sum.y, f.z, l);
+                        }
+                        tmem_st16(tm_s + 16 * q, u);  // (below the scores that are still to come)
+                    }
+                    if (j + 1 == nt) {  // the row's sum, through a column that P leaves free, before the next item's scores can come
+                        tmem_st1(tm_s + 32, l);
+                        tmem_st_wait();
+                        tc_fence_before();
+                        named_bar_sync(pair, 64);
+                        tc_fence_after();
+                        l += tmem_ld1((tm_s ^ 64) + 32);
+                        tc_fence_before();
+                        named_bar_sync(pair, 64);
+                    }
                     tmem_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(q ? &bar_pb[w] : &bar_pa[w]);
+                    if (lane == 0) mbar_arrive(half ? &bar_pb[w] : &bar_pa[w]);
                 }
-            }
-            if (!ok) break;
-            // ── output ──
-            if (it.nt > 0) {
+                if (!ok) break;
+                // ── output ──
                 if (!(ok = attn_wait(&bar_o[w], ph_o, abort_flag))) break;
                 ph_o ^= 1;
                 tc_fence_after();
-            }
-            if (!dead) {
-                const bool mine = wrow + lane < it.n_packed;
-                const size_t row = (size_t)tok * a.n_q + head, part = (size_t)it.split * a.n_rows * a.n_q + row;
-                const float inv = l > 0.f ? 1.f / l : 0.f;
-                if (mine) {
-                    const float lw = l > 0.f ? M + log2f(l) : -INFINITY;
-                    if (parts.o) parts.w[part] = lw;
-                    else if (a.lse) a.lse[row] = lw * kLn2;
-                }
-#pragma unroll
-                for (int i = 0; i < HD / 16; i++) {
-                    uint32_t o[16], u[8];
-                    if (it.nt > 0) {
+                if (!dead) {
+                    const int R = it->row0 + in_tile + lane;
+                    const bool mine = R < it->n_packed;
+                    const int t = R / rep, tok = it->r0 + t, head = it->kvh * rep + R - t * rep;
+                    const size_t row = (size_t)tok * a.n_q + head, part = (size_t)it->split * a.n_rows * a.n_q + row;
+                    const float inv = l > 0.f ? 1.f / l : 0.f;
+                    if (half == 0 && mine) {
+                        const float lw = l > 0.f ? M + log2f(l) : -INFINITY;
+                        if (parts.o) parts.w[part] = lw;
+                        else if (a.lse) a.lse[row] = lw * kLn2;
+                    }
+#pragma unroll 1
+                    for (int i = 0; i < HD / 32; i++) {
+                        uint32_t o[16], u[8];
                         tmem_ld16(tm_o + 16 * i, o);
                         tmem_ld_wait(o);
-                    }
-                    if (!mine) continue;
-                    if (parts.o) {
+                        if (!mine) continue;
+                        const int d0 = half * (HD / 2) + 16 * i;
+                        if (parts.o) {
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
+                            for (int h = 0; h < 2; h++) {
 #pragma unroll
-                            for (int e = 0; e < 8; e++) u[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[8 * h + e]) * inv) : 0;
-                            store_row32(parts.o + part * HD + 16 * i + 8 * h, 16, u);
+                                for (int e = 0; e < 8; e++) u[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[8 * h + e]) * inv) : 0;
+                                store_row32(parts.o + part * HD + d0 + 8 * h, 16, u);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; e++) reinterpret_cast<T *>(u)[e] = from_f32<T>(l > 0.f ? __uint_as_float(o[e]) * inv : 0.f);
+                            store_row32(reinterpret_cast<T *>(a.out) + tok * a.out_tok + head * a.out_head + d0, out_align, u);
                         }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) reinterpret_cast<T *>(u)[e] = from_f32<T>(l > 0.f ? __uint_as_float(o[e]) * inv : 0.f);
-                        store_row32(reinterpret_cast<T *>(a.out) + tok * a.out_tok + head * a.out_head + 16 * i, out_align, u);
                     }
+                    tc_fence_before();
                 }
-                tc_fence_before();
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[k & (kTcItems - 1)]);
         }
         if (!ok && lane == 0 && status) atomicOr(status, DFB_STAT_TIMEOUT);
-    } else if (warp < 12) {
+    } else if (warp < 20) {
         // ── converters ──
-        const int cw = warp - 8;
-        int n = 0, odd = 0, seen[2] = {0, 0};  // code tiles so far, parity of the item, score phases of each row tile so far
+        const int cw = warp - 16;
+        int n = 0, odd = 0;  // code tiles so far, parity of the item
         bool ok = true;
-        for (int idx = blockIdx.x; ok && idx < grid.items; idx += gridDim.x) {
-            if (!tc_item(c, a, parts, grid, rep, idx, status, it)) continue;
-            odd ^= it.nt > 0;
-            for (int i = 0; ok && i < 2 * it.nt; i++, n++) {
+        for (int k = 0; ok; k++) {
+            const volatile TcItem *it = items + (k & (kTcItems - 1));
+            if (!(ok = attn_wait(&item_full[k & (kTcItems - 1)], (k / kTcItems) & 1, abort_flag))) break;
+            const int nt = it->nt;
+            if (nt < 0) break;
+            odd ^= 1;
+            for (int i = 0; ok && i < 2 * nt; i++, n++) {
                 if (i == 1) {
-                    // the item's queries as f16, scaled by a power of two: a quarter of each row tile per
-                    // warp, once the last scores of the item before are there
-                    constexpr int LPR = HD / 8, RPI = 32 / LPR, NL = 8;  // lanes of a row (16 bytes each), rows of one load, loads in flight
-                    for (int w = 0; ok && w < (it.two ? 2 : 1); w++) {
-                        if (seen[w] > 0 && !(ok = attn_wait(&bar_s[w], (seen[w] - 1) & 1, abort_flag))) break;
-                        seen[w] += it.nt;
-                        const int ch = lane % LPR;
-#pragma unroll 1
-                        for (int b = 0; b < 32; b += NL * RPI) {
-                            uint4 raw[NL];
-                            const T *from[NL];
+                    // the item's queries as f16: a quarter of each row tile per warp, once the last scores of the
+                    // item before are there; copied into place and converted there
+                    constexpr int LPR = HD / 8, RPI = 32 / LPR, NI = 32 / RPI;  // lanes of a row (16 bytes each), rows of one round, rounds
+                    const int ch = lane % LPR, n_packed = it->n_packed;
+                    uint8_t *dst = sm + L::q_off + (ch / 8) * 16384;
+                    const int n_w = it->row0 + 128 < n_packed ? 2 : 1;
+                    const int last = (n >> 1) - 1;  // the tile before the item: event `last` says that its scores are there
+                    if (last >= 0 && !(ok = attn_wait(&freed[last & 1], (last >> 1) & 1, abort_flag))) break;
+                    for (int w = 0; w < n_w; w++) {
+#pragma unroll 4
+                        for (int q = 0; q < NI; q++) {
+                            const int rt = cw * 32 + q * RPI + lane / LPR;
+                            // (a row that does not exist is read as the last one: what comes of it is not stored)
+                            const int r = min(it->row0 + w * 128 + rt, n_packed - 1), t = r / rep;
+                            const T *from = reinterpret_cast<const T *>(a.q) + (it->r0 + t) * a.q_tok + (it->kvh * rep + r - t * rep) * a.q_head + 8 * ch;
+                            uint8_t *at = dst + w * L::q + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4);
+                            if (vec) cp_async16(at, from);
+                            else
 #pragma unroll
-                            for (int i = 0; i < NL; i++) {
-                                // (a row that does not exist is read as the last one: what comes of it is not stored)
-                                const int r = min(it.row0 + w * 128 + cw * 32 + b + i * RPI + lane / LPR, it.n_packed - 1), t = r / rep;
-                                from[i] = reinterpret_cast<const T *>(a.q) + (it.sq.r0 + t) * a.q_tok + (it.kvh * rep + r - t * rep) * a.q_head + 8 * ch;
-                            }
-                            if (vec) {
-#pragma unroll
-                                for (int i = 0; i < NL; i++) raw[i] = *reinterpret_cast<const uint4 *>(from[i]);
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < NL; i++)
-#pragma unroll
-                                    for (int e = 0; e < 8; e++) reinterpret_cast<T *>(&raw[i])[e] = from[i][e];
-                            }
-                            float up[NL];
-#pragma unroll
-                            for (int i = 0; i < NL; i++) up[i] = 1.f;
-                            if constexpr (!std::is_same<T, __half>::value) {
-                                float mx[NL];
-#pragma unroll
-                                for (int i = 0; i < NL; i++) {
-                                    mx[i] = 0.f;
-#pragma unroll
-                                    for (int e = 0; e < 8; e++) mx[i] = fmaxf(mx[i], fabsf(to_f32<T>(reinterpret_cast<const T *>(&raw[i])[e])));
-                                }
-#pragma unroll
-                                for (int o = 1; o < LPR; o <<= 1)
-#pragma unroll
-                                    for (int i = 0; i < NL; i++) mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
-#pragma unroll
-                                for (int i = 0; i < NL; i++) {
-                                    const int e = (int)(__float_as_uint(mx[i]) >> 23) - 127;
-                                    const int eu = mx[i] > 0.f && mx[i] < INFINITY ? min(max(-e, -126), 60) : 0;
-                                    up[i] = exp2i(eu);
-                                    if (ch == 0) reinterpret_cast<int8_t *>(sm + L::crow_off)[odd * kTcRows + w * 128 + cw * 32 + b + i * RPI + lane / LPR] = (int8_t)-eu;
-                                }
-                            }
-#pragma unroll
-                            for (int i = 0; i < NL; i++) {
-                                float x[8];
-                                const int rt = cw * 32 + b + i * RPI + lane / LPR;
-                                const float f = a.scale < 0.f ? -up[i] : up[i];  // a negative scale turns q's sign: the scores' factors stay positive
-#pragma unroll
-                                for (int e = 0; e < 8; e++) x[e] = to_f32<T>(reinterpret_cast<const T *>(&raw[i])[e]) * f;
-                                uint4 u;
-                                u.x = pack_f16(x[0], x[1]); u.y = pack_f16(x[2], x[3]);
-                                u.z = pack_f16(x[4], x[5]); u.w = pack_f16(x[6], x[7]);
-                                *reinterpret_cast<uint4 *>(sm + L::q_off + w * L::q + (ch / 8) * 16384 + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4)) = u;
-                            }
+                                for (int e = 0; e < 8; e++) reinterpret_cast<T *>(at)[e] = from[e];
                         }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar_q[w]);
                     }
-                    if (!ok) break;
+                    cp_async_commit();
+                    cp_async_wait<0>();
+                    // bf16 rows whose largest value f16 holds with room to spare above and below are converted as
+                    // they are (what f16's subnormals then cut off is below 2^-21 of it), others are scaled to
+                    // [1, 2) first; a negative softmax scale turns q's sign: the scores' factors stay positive
+                    if (!std::is_same<T, __half>::value || a.scale < 0.f)
+                        for (int w = 0; w < n_w; w++)
+#pragma unroll 2
+                            for (int q = 0; q < NI; q++) {
+                                const int rt = cw * 32 + q * RPI + lane / LPR;
+                                uint4 *at = reinterpret_cast<uint4 *>(dst + w * L::q + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4));
+                                uint4 u = *at;
+                                if constexpr (!std::is_same<T, __half>::value) {
+                                    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
+                                    const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+                                    const uint32_t mb = *reinterpret_cast<const uint32_t *>(&m);
+                                    uint32_t mx = max(mb & 0xffffu, mb >> 16);  // bits of a magnitude: ordered like the magnitudes
+#pragma unroll
+                                    for (int o = 1; o < LPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                                    const int e = (int)(mx >> 7) - 127;  // (128: inf or NaN)
+                                    const int eu = mx != 0 && e < 128 && (e < -3 || e > 13) ? min(max(-e, -126), 60) : 0;
+                                    if (ch == 0) reinterpret_cast<int8_t *>(sm + L::crow_off)[odd * kTcRows + w * 128 + rt] = (int8_t)-eu;
+                                    const float f = exp2i(eu);
+                                    const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+                                    uint32_t o[4];
+#pragma unroll
+                                    for (int p = 0; p < 4; p++) o[p] = pack_f16(__uint_as_float(v[p] << 16) * f, __uint_as_float(v[p] & 0xffff0000u) * f);
+                                    u = make_uint4(o[0], o[1], o[2], o[3]);
+                                }
+                                if (a.scale < 0.f) { u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u; }
+                                *at = u;
+                            }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0)
+                        for (int w = 0; w < n_w; w++) mbar_arrive(&bar_q[w]);
                 }
                 const int rs = n % kTcRaw, cs = n % kTcSlots, g = n >> 1;
                 if (!(ok = attn_wait(&raw_full[rs], (n / kTcRaw) & 1, abort_flag))) break;
                 // V(g) and K(g + 1) are freed together, by event g + 1 (K(0) by event 0); events alternate
-                // between two barriers, and the issuer is never two events ahead of this wait
+                // between two barriers, and the issuer is never two events ahead of this wait (event g + 1
+                // needs K(g + 1), which waited for event g)
                 const int ev = (n - kTcSlots + 1) >> 1;
                 if (n >= kTcSlots && !(ok = attn_wait(&freed[ev & 1], (ev >> 1) & 1, abort_flag))) break;
                 const uint8_t *src = sm + L::raw_off + rs * L::raw;
                 uint8_t *dst = sm + L::slot_off + cs * L::slot;
                 const float4 *gs = sc + (g & 3) * 8;
-                const int left = it.kend - (it.t0 + (i >> 1)) * kTcKeys;
+                const int left = it->kend - (it->t0 + (i >> 1)) * kTcKeys;
                 const bool edge = (i & 1) && (left < kTcKeys || gs[0].w != 0.f);
                 // eight lanes of a shared-memory phase take four 16-byte columns of two rows whose swizzles
                 // do not meet, for the loads and for the stores
@@ -515,119 +559,158 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&conv_full[cs]);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[k & (kTcItems - 1)]);
         }
-    } else if (warp == 12) {
+    } else if (warp == 20) {
         // ── MMA issuer ──
         const uint32_t id_s = idesc_f16(128, kTcKeys), id_o = idesc_f16(128, HD) | (1u << 16);  // V is MN-major
         const uint32_t base = smem_u32(sm);
         const uint64_t dq = sw128_desc(base + L::q_off), dk = sw128_desc(base + L::slot_off), dv = mn128_desc(base + L::slot_off, 16384);
-        // Every instruction of the issuing thread beside an MMA costs about ten cycles (its scheduler has
-        // five busy warps): the loop over an item's tiles holds nothing but waits, MMAs and commits.
+        // An MMA takes 64 cycles and an instruction of this warp about ten (its scheduler has three busy
+        // warps): the warp stays whole (uniform registers), descriptors differ by constants, and the loop
+        // over an item's tiles holds nothing but waits, MMAs and commits.
         bool ok = true;
         auto ready = [&](uint64_t *b, uint32_t ph) {
-            ok = ok && thread_wait(b, ph, abort_flag);
+            ok = ok && attn_wait(b, ph, abort_flag);
             tc_fence_after();
         };
-        auto value_of = [&](int g) { return dv + (g & 1 ? 3 : 1) * (L::slot >> 4); };  // V(g) is in slot (2 g + 1) % 4
-        auto key_of = [&](int g) { return dk + (g & 1 ? 2 : 0) * (L::slot >> 4); };    // K(g) in slot 2 g % 4
-        auto wait_value = [&](int g) { ready(&conv_full[g & 1 ? 3 : 1], (g >> 1) & 1); };
-        auto wait_key = [&](int g) { ready(&conv_full[g & 1 ? 2 : 0], (g >> 1) & 1); };
-        static_assert(kTcSlots == 4, "slots of K and V");
-        uint32_t ph_p[2] = {0, 0}, ph_q[2] = {0, 0};
-        auto value = [&](int w, uint64_t d, bool first) {
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                ready(half ? &bar_pb[w] : &bar_pa[w], ph_p[w]);
-                if (!ok) return;
-#pragma unroll
-                for (int i = 0; i < kTcKeys / 32; i++)
-                    mma1_f16_ts(tmem + 256 + w * 128, tmem + w * 128 + 32 * half + 8 * i, d + (2048 >> 4) * (4 * half + i), id_o, !(first && half == 0 && i == 0));
-            }
+        // K(g) is in slot 2 g % 3, V(g) in slot (2 g + 1) % 3; MOD: g % 3
+        static_assert(kTcSlots == 3, "slots");
+        uint32_t ph_p[2] = {0, 0}, ph_q[2] = {0, 0}, ph_c[3] = {0, 0, 0};
+        auto filled = [&](auto S) {
+            ready(&conv_full[decltype(S)::value], ph_c[decltype(S)::value]);
+            ph_c[decltype(S)::value] ^= 1;
+        };
+        // P V of row tile W from the values of a tile
+        auto value = [&](auto W, auto MOD, bool first) {
+            constexpr int w = decltype(W)::value;
+            const uint64_t d = dv + (2 * decltype(MOD)::value + 1) % 3 * (L::slot >> 4);
+            ready(&bar_pa[w], ph_p[w]);
+            ready(&bar_pb[w], ph_p[w]);
+            if (ok && elect_one())
+                unrolled<kTcKeys / 16>([&](auto I) {
+                    constexpr int i = decltype(I)::value;
+                    mma1_f16_ts<256 + w * 128, w * 128 + 64 * (i >> 2) + 8 * (i & 3)>(d + (2048 >> 4) * i, id_o, i > 0 || !first);
+                });
             ph_p[w] ^= 1;
         };
-        auto score = [&](int w, uint64_t d) {
-            if (!ok) return;
-#pragma unroll
-            for (int k = 0; k < HD / 16; k++) {
-                const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                mma1_f16_ss(tmem + w * 128, dq + w * (L::q >> 4) + off, d + off, id_s, k > 0);
+        auto score = [&](auto W, auto MOD) {
+            constexpr int w = decltype(W)::value;
+            const uint64_t d = dk + 2 * decltype(MOD)::value % 3 * (L::slot >> 4);
+            if (ok && elect_one()) {
+                unrolled<HD / 16>([&](auto K) {
+                    constexpr int k = decltype(K)::value, off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                    mma1_f16_ss<w * 128, (k > 0)>(dq + w * (L::q >> 4) + off, d + off, id_s);
+                });
+                mma1_commit(&bar_s[w]);
             }
-            mma1_commit(&bar_s[w]);
+        };
+        auto commit = [&](uint64_t *b) {
+            if (ok && elect_one()) mma1_commit(b);
         };
         auto queries = [&](int w) {
             ready(&bar_q[w], ph_q[w]);
             ph_q[w] ^= 1;
         };
-        int idx = (int)blockIdx.x - (int)gridDim.x, g = 0;
-        auto next = [&] {  // the next item with keys (all lanes)
-            do idx += gridDim.x;
-            while (idx < grid.items && !(tc_item(c, a, parts, grid, rep, idx, status, it) && it.nt > 0));
-            return idx < grid.items;
+        int k = -1, g = 0, mod = 0, nt_next = 0;
+        bool two_next = false;
+        auto next = [&] {
+            if (k >= 0 && lane == 0) mbar_arrive(&item_empty[k & (kTcItems - 1)]);
+            k++;
+            if (!(ok = attn_wait(&item_full[k & (kTcItems - 1)], (k / kTcItems) & 1, abort_flag))) return false;
+            const volatile TcItem *it = items + (k & (kTcItems - 1));
+            nt_next = it->nt;
+            two_next = it->row0 + 128 < it->n_packed;
+            __syncwarp();
+            return nt_next > 0;
         };
         bool have = next();
-        if (have && lane == 0) {
-            wait_key(0);
+        if (have) {
+            filled(Int<0>());
             queries(0);
-            score(0, key_of(0));
-            if (it.two) {
+            score(Int<0>(), Int<0>());
+            if (two_next) {
                 queries(1);
-                score(1, key_of(0));
+                score(Int<1>(), Int<0>());
             }
-            if (ok) mma1_commit(&freed[0]);
+            commit(&freed[0]);
         }
-        while (have) {
-            const int nt = it.nt;
-            const bool two = it.two;
+        while (have && ok) {
+            const int nt = nt_next;
+            const bool two = two_next;
             have = next();
-            if (lane == 0 && ok) {
-                for (int t = 0; t + 1 < nt && ok; t++, g++) {
-                    const uint64_t d = value_of(g), dn = key_of(g + 1);
-                    wait_value(g);
-                    value(0, d, t == 0);
-                    wait_key(g + 1);
-                    score(0, dn);
+            // tile t (MOD: its index g % 3) and the scores of the one after it
+            auto tile = [&](auto MOD, int t) {
+                using Next = Int<(decltype(MOD)::value + 1) % 3>;
+                using KeySlot = Int<2 * Next::value % 3>;
+                uint64_t *event = &freed[(g + 1) & 1];
+                filled(Int<(2 * decltype(MOD)::value + 1) % 3>());
+                value(Int<0>(), MOD, t == 0);
+                if (t + 1 < nt) {
+                    filled(KeySlot());
+                    score(Int<0>(), Next());
                     if (two) {
-                        value(1, d, t == 0);
-                        score(1, dn);
+                        value(Int<1>(), MOD, t == 0);
+                        score(Int<1>(), Next());
                     }
-                    if (ok) mma1_commit(&freed[(g + 1) & 1]);
-                }
-                const uint64_t d = value_of(g), dn = key_of(g + 1);  // the item's last tile, the next one's first
-                wait_value(g);
-                value(0, d, nt == 1);
-                if (ok) mma1_commit(&bar_o[0]);
-                if (have) {
-                    wait_key(g + 1);
-                    queries(0);
-                    score(0, dn);
-                }
-                if (two) {
-                    value(1, d, nt == 1);
-                    if (ok) mma1_commit(&bar_o[1]);
-                }
-                if (have) {
-                    if (it.two) {
-                        queries(1);
-                        score(1, dn);
+                    commit(event);
+                } else {  // the item's last tile, the next one's first
+                    commit(&bar_o[0]);
+                    if (have) {
+                        filled(KeySlot());
+                        queries(0);
+                        score(Int<0>(), Next());
                     }
-                    if (ok) mma1_commit(&freed[(g + 1) & 1]);  // (the CTA's last commits are bar_o's, which the softmax warps wait for)
+                    if (two) {
+                        value(Int<1>(), MOD, t == 0);
+                        commit(&bar_o[1]);
+                    }
+                    if (have) {
+                        if (two_next) {
+                            queries(1);
+                            score(Int<1>(), Next());
+                        }
+                        commit(event);  // (the CTA's last commits are bar_o's, which the softmax warps wait for)
+                    }
                 }
-                g++;
+            };
+            for (int t = 0; t < nt && ok; t++, g++, mod = mod == 2 ? 0 : mod + 1) {
+                if (mod == 0) tile(Int<0>(), t);
+                else if (mod == 1) tile(Int<1>(), t);
+                else tile(Int<2>(), t);
             }
-            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
         }
-        if (!ok && lane == 0) {  // let what was issued end before TMEM is freed
+        if (!ok && elect_one()) {  // let what was issued end before TMEM is freed
             mma1_commit(bar_drain);
             spin_bounded(bar_drain, 0);
         }
         __syncwarp();
-    } else if (warp == 13) {
+    } else if (warp == 21) {
         // ── loader ──
         const int box = min(c.page, kKeyTile), sh_box = __ffs(box) - 1, nb = kTcKeys >> sh_box, sh_page = __ffs(c.page) - 1;
-        int n = 0;
+        int n = 0, k = 0, idx = (int)blockIdx.x - (int)gridDim.x;
         bool ok = true;
-        for (int idx = blockIdx.x; ok && idx < grid.items; idx += gridDim.x) {
-            if (!tc_item(c, a, parts, grid, rep, idx, status, it)) continue;
+        // The next item, published one ahead of its loads: the issuer looks at it while it works on the one before.
+        auto publish = [&](TcItem &t) {
+            do idx += gridDim.x;
+            while (idx < grid.items && !(tc_item(c, a, parts, grid, rep, idx, status, t) && t.nt > 0));
+            if (idx >= grid.items) t.nt = -1;
+            if (k >= kTcItems && !(ok = attn_wait(&item_empty[k & (kTcItems - 1)], (k / kTcItems - 1) & 1, abort_flag))) return;
+            if (lane == 0) {
+                volatile TcItem *o = reinterpret_cast<volatile TcItem *>(sm + L::item_off) + (k & (kTcItems - 1));
+                o->s = t.s; o->kvh = t.kvh; o->split = t.split; o->r0 = t.r0; o->len = t.len; o->row0 = t.row0;
+                o->n_packed = t.n_packed; o->kend = t.kend; o->t0 = t.t0; o->nt = t.nt;
+                mbar_arrive(&item_full[k & (kTcItems - 1)]);
+            }
+            __syncwarp();
+            k++;
+        };
+        TcItem it, after;
+        publish(it);
+        while (ok && it.nt > 0) {
+            publish(after);
+            if (!ok) break;
             int pid = 0;
             float ks = 1.f, vs = 1.f;
             for (int i = 0; i < 2 * it.nt; i++, n++) {
@@ -670,14 +753,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive_expect_tx(&raw_full[rs], n_ok * box * HD);
             }
+            it = after;
         }
         if (*abort_flag)  // let the copies in flight land before the block goes
             for (int i = max(0, n - kTcRaw); i < n; i++) spin_bounded(&raw_full[i % kTcRaw], (i / kTcRaw) & 1);
     }
+    if (warp == 22) {
+        // ── rows of items without keys ──
+        TcItem it;
+        for (int idx = blockIdx.x; idx < grid.items; idx += gridDim.x) {
+            if (!tc_item(c, a, parts, grid, rep, idx, status, it) || it.nt > 0) continue;
+            for (int r = it.row0; r < min(it.row0 + kTcRows, it.n_packed); r++) {
+                const int t = r / rep, tok = it.r0 + t, head = it.kvh * rep + r - t * rep;
+                const size_t row = (size_t)tok * a.n_q + head;
+                if (parts.o) {
+                    if (lane == 0) parts.w[(size_t)it.split * a.n_rows * a.n_q + row] = -INFINITY;
+                    continue;
+                }
+                if (a.lse && lane == 0) a.lse[row] = -INFINITY;
+                for (int d = lane; d < HD; d += 32) reinterpret_cast<T *>(a.out)[tok * a.out_tok + head * a.out_head + d] = from_f32<T>(0.f);
+            }
+        }
+    }
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 20) {
         tc_fence_after();
-        tmem_dealloc1(tmem, 512);
+        tmem_dealloc1((uint32_t)shared_i[1], 512);
     }
 }
 

@@ -367,7 +367,8 @@ def kill_tail(c, lens):
     (1, 1, 64, 16, [1], [1]),
     (4, 28, 128, 64, [5000, 1], [1, 1]),
     (1, 32, 64, 32, [1000], [130]),
-], ids=["decode", "tiny-p16", "gqa7-p32", "mha-p128", "gqa8-hd64", "long-rows", "one-one", "decode-2", "mqa32"])
+    (5, 10, 128, 64, [1500, 3, 0, 900, 128, 129] * 7, [260, 3, 2, 70, 129, 40] * 7),
+], ids=["decode", "tiny-p16", "gqa7-p32", "mha-p128", "gqa8-hd64", "long-rows", "one-one", "decode-2", "mqa32", "many-items"])
 def test_attention(ops, dtype, n_kv, n_q, hd, page, lens, counts):
     most = max(1, max(-(-m // page) for m in lens))
     c = kill_tail(make_cache(ops, len(lens), n_kv, hd, page, most, seed=7), lens)
