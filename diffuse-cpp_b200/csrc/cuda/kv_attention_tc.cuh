@@ -46,7 +46,7 @@ struct TcSmem {
     static constexpr int raw = kTcKeys * HD;
     static constexpr int q_off = 0, slot_off = 2 * q, raw_off = slot_off + kTcSlots * slot, sc_off = raw_off + kTcRaw * raw;
     static constexpr int bar_off = sc_off + 4 * 8 * 16;
-    static constexpr int n_bars = 2 * kTcRaw + kTcSlots + 13 + 2 * kTcItems;
+    static constexpr int n_bars = 2 * kTcRaw + kTcSlots + 15 + 2 * kTcItems;
     static constexpr int item_off = bar_off + n_bars * 8 + 16;
     static constexpr int crow_off = item_off + kTcItems * (int)sizeof(TcItem);
     static constexpr int bytes = 1024 + crow_off + 2 * kTcRows;
@@ -167,6 +167,10 @@ __device__ __forceinline__ uint64_t mn128_desc(uint32_t smem_addr, uint32_t bloc
     return d;
 }
 
+// One arrival on the mbarrier once this thread's cp.async so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // 32 bytes to global memory in one store.
 __device__ __forceinline__ void store32(void *p, const uint32_t (&u)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
@@ -224,7 +228,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     float4 *sc = reinterpret_cast<float4 *>(sm + L::sc_off);  // [tile & 3][8 runs of 16 keys] ks, log2 vs, 1 / vs, any absent
     uint64_t *bars = reinterpret_cast<uint64_t *>(sm + L::bar_off);
     uint64_t *raw_full = bars, *raw_empty = raw_full + kTcRaw, *conv_full = raw_empty + kTcRaw, *freed = conv_full + kTcSlots;
-    uint64_t *bar_s = freed + 2, *bar_pa = bar_s + 2, *bar_pb = bar_pa + 2, *bar_o = bar_pb + 2, *bar_q = bar_o + 2, *item_full = bar_q + 2,
+    uint64_t *bar_s = freed + 2, *bar_pa = bar_s + 2, *bar_pb = bar_pa + 2, *bar_o = bar_pb + 2, *bar_q = bar_o + 2, *bar_raw_q = bar_q + 2, *item_full = bar_raw_q + 2,
              *item_empty = item_full + kTcItems, *bar_drain = item_empty + kTcItems;
     int *shared_i = reinterpret_cast<int *>(bars + L::n_bars);  // abort flag, TMEM address
     volatile int *abort_flag = shared_i;
@@ -244,7 +248,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar_pb[i], 4);
             mbar_init(&freed[i], 1);
             mbar_init(&bar_o[i], 1);
-            mbar_init(&bar_q[i], 4);
+            mbar_init(&bar_q[i], 8);
+            mbar_init(&bar_raw_q[i], 128);
         }
         for (int i = 0; i < kTcItems; i++) {
             mbar_init(&item_full[i], 1);
@@ -267,17 +272,75 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t tm_s = tmem + w * 128 + 64 * half + ((uint32_t)(warp & 3) << 21);  // this half's scores; 64 ^: the other's
         const uint32_t tm_o = tmem + 256 + w * 128 + half * (HD / 2) + ((uint32_t)(warp & 3) << 21);  // this half of the dimensions
         const int in_tile = w * 128 + (warp & 3) * 32;  // the warp's first row in the item
-        uint32_t ph_s = 0, ph_o = 0, odd = 0;
+        uint32_t ph_s = 0, ph_o = 0, ph_q = 0;
         int g = 0;  // key tiles of the CTA so far
         bool ok = true;
-        for (int k = 0;; k++) {
+        // Half of the warp's 32 query rows of item k as f16 operands.  bf16 rows whose largest value f16
+        // holds with room to spare above and below are converted as they are (what f16's subnormals then cut
+        // off is below 2^-21 of it), others are scaled to [1, 2) first; a negative softmax scale turns q's
+        // sign: the scores' factors stay positive.
+        auto queries = [&](int k) {
             const volatile TcItem *it = items + (k & (kTcItems - 1));
-            if (!(ok = attn_wait(&item_full[k & (kTcItems - 1)], (k / kTcItems) & 1, abort_flag))) break;
+            if (!(ok = attn_wait(&item_full[k & (kTcItems - 1)], (k / kTcItems) & 1, abort_flag))) return;
+            if (it->nt < 0 || (w == 1 && it->row0 + 128 >= it->n_packed)) return;
+            if (!(ok = attn_wait(&bar_raw_q[w], ph_q, abort_flag))) return;
+            ph_q ^= 1;
+            constexpr int LPR = HD / 8, RPI = 32 / LPR;  // lanes of a row (16 bytes each), rows of one round
+            const int ch = lane % LPR;
+            if ((!std::is_same<T, __half>::value || a.scale < 0.f) && it->row0 + in_tile < it->n_packed) {
+#pragma unroll 2
+                for (int x = 0; x < 16 / RPI; x++) {
+                    const int rt = (warp & 3) * 32 + half * 16 + x * RPI + lane / LPR;
+                    uint4 *at = reinterpret_cast<uint4 *>(sm + L::q_off + w * L::q + (ch / 8) * 16384 + rt * 128 + (((ch ^ rt) & 7) << 4));
+                    uint4 u = *at;
+                    if constexpr (!std::is_same<T, __half>::value) {
+                        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
+                        const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+                        const uint32_t mb = *reinterpret_cast<const uint32_t *>(&m);
+                        uint32_t mx = max(mb & 0xffffu, mb >> 16);  // bits of a magnitude: ordered like the magnitudes
+                        int eu = 0;
+                        // all rows of the round within [2^-3, 2^14): no lane above, one lane of each row above the lower end
+                        const uint32_t above = __ballot_sync(0xffffffffu, mx >= (124u << 7));
+                        bool plain = !__any_sync(0xffffffffu, mx >= (141u << 7));
+#pragma unroll
+                        for (int r = 0; r < RPI; r++) plain = plain && (above >> (r * LPR) & ((1u << LPR) - 1)) != 0;
+                        if (!plain) {
+#pragma unroll
+                            for (int o = 1; o < LPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            const int e = (int)(mx >> 7) - 127;  // (128: inf or NaN)
+                            eu = mx != 0 && e < 128 && (e < -3 || e > 13) ? min(max(-e, -126), 60) : 0;
+                        }
+                        if (ch == 0) reinterpret_cast<int8_t *>(sm + L::crow_off)[(k & 1) * kTcRows + w * 128 + rt] = (int8_t)-eu;
+                        const uint32_t v[4] = {u.x, u.y, u.z, u.w};
+                        uint32_t o[4];
+                        const float f = exp2i(eu);
+#pragma unroll
+                        for (int p = 0; p < 4; p++) {
+                            float lo = __uint_as_float(v[p] << 16), hi = __uint_as_float(v[p] & 0xffff0000u);
+                            if (!plain) {
+                                lo *= f;
+                                hi *= f;
+                            }
+                            o[p] = pack_f16(lo, hi);
+                        }
+                        u = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                    if (a.scale < 0.f) { u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u; }
+                    *at = u;
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar_q[w]);
+        };
+        queries(0);
+        for (int k = 0; ok; k++) {
+            const volatile TcItem *it = items + (k & (kTcItems - 1));  // (published: queries(k) has waited)
             const int nt = it->nt;
             if (nt < 0) break;
-            odd ^= 1;
             if (w == 1 && it->row0 + 128 >= it->n_packed) {  // no row tile 1
                 g += nt;
+                queries(k + 1);
             } else {
                 const bool dead = it->row0 + in_tile >= it->n_packed;  // no row of this warp exists: no one reads what comes of its lanes
                 float cr = fabsf(a.scale) * kLog2e, M = -INFINITY, l = 0.f;
@@ -298,7 +361,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_fence_after();
                     // exponents of the queries' scales, by the parity of the item: one is written while the other may still be read
                     if (!std::is_same<T, __half>::value && j == 0)
-                        cr *= exp2i(reinterpret_cast<const int8_t *>(sm + L::crow_off)[odd * kTcRows + in_tile + lane]);
+                        cr *= exp2i(reinterpret_cast<const int8_t *>(sm + L::crow_off)[(k & 1) * kTcRows + in_tile + lane]);
                     const float4 *gs = sc + (g & 3) * 8 + 4 * half;
                     const bool cut = __any_sync(0xffffffffu, left < 64 || gs[0].w != 0.f);  // (keys of a bad page: rare)
                     // 32 scores at a time: 64 would spill, and the memory behind a spill is L2 (227 KB of shared
@@ -396,8 +459,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (lane == 0) mbar_arrive(half ? &bar_pb[w] : &bar_pa[w]);
                 }
                 if (!ok) break;
+                queries(k + 1);  // (under the last tile's P V)
                 // ── output ──
-                if (!(ok = attn_wait(&bar_o[w], ph_o, abort_flag))) break;
+                if (!ok || !(ok = attn_wait(&bar_o[w], ph_o, abort_flag))) break;
                 ph_o ^= 1;
                 tc_fence_after();
                 if (!dead) {
@@ -441,74 +505,37 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     } else if (warp < 20) {
         // ── converters ──
         const int cw = warp - 16;
-        int n = 0, odd = 0;  // code tiles so far, parity of the item
+        int n = 0;  // code tiles so far
         bool ok = true;
         for (int k = 0; ok; k++) {
             const volatile TcItem *it = items + (k & (kTcItems - 1));
             if (!(ok = attn_wait(&item_full[k & (kTcItems - 1)], (k / kTcItems) & 1, abort_flag))) break;
             const int nt = it->nt;
             if (nt < 0) break;
-            odd ^= 1;
             for (int i = 0; ok && i < 2 * nt; i++, n++) {
-                if (i == 1) {
-                    // the item's queries as f16: a quarter of each row tile per warp, once the last scores of the
-                    // item before are there; copied into place and converted there
-                    constexpr int LPR = HD / 8, RPI = 32 / LPR, NI = 32 / RPI;  // lanes of a row (16 bytes each), rows of one round, rounds
-                    const int ch = lane % LPR, n_packed = it->n_packed;
-                    uint8_t *dst = sm + L::q_off + (ch / 8) * 16384;
-                    const int n_w = it->row0 + 128 < n_packed ? 2 : 1;
+                if (i == 0) {
+                    // the item's queries into place, once the last scores of the item before are there; the
+                    // softmax warps turn them into operands when they have landed
+                    constexpr int LPR = HD / 8, RPI = 32 / LPR;  // lanes of a row (16 bytes each), rows of one round
+                    const int ch = lane % LPR, n_packed = it->n_packed, row0 = it->row0 + cw * 32 + lane / LPR, n_w = it->row0 + 128 < n_packed ? 2 : 1;
+                    const T *q = reinterpret_cast<const T *>(a.q) + it->r0 * a.q_tok + it->kvh * rep * a.q_head + 8 * ch;
                     const int last = (n >> 1) - 1;  // the tile before the item: event `last` says that its scores are there
                     if (last >= 0 && !(ok = attn_wait(&freed[last & 1], (last >> 1) & 1, abort_flag))) break;
                     for (int w = 0; w < n_w; w++) {
+                        uint8_t *dst = sm + L::q_off + w * L::q + (ch / 8) * 16384 + (cw * 32 + lane / LPR) * 128;
 #pragma unroll 4
-                        for (int q = 0; q < NI; q++) {
-                            const int rt = cw * 32 + q * RPI + lane / LPR;
+                        for (int x = 0; x < 32 / RPI; x++) {
                             // (a row that does not exist is read as the last one: what comes of it is not stored)
-                            const int r = min(it->row0 + w * 128 + rt, n_packed - 1), t = r / rep;
-                            const T *from = reinterpret_cast<const T *>(a.q) + (it->r0 + t) * a.q_tok + (it->kvh * rep + r - t * rep) * a.q_head + 8 * ch;
-                            uint8_t *at = dst + w * L::q + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4);
+                            const int r = min(row0 + w * 128 + x * RPI, n_packed - 1), t = r / rep;
+                            const T *from = q + t * a.q_tok + (r - t * rep) * a.q_head;
+                            uint8_t *at = dst + x * RPI * 128 + (((ch ^ (cw * 32 + lane / LPR + x * RPI)) & 7) << 4);
                             if (vec) cp_async16(at, from);
                             else
 #pragma unroll
                                 for (int e = 0; e < 8; e++) reinterpret_cast<T *>(at)[e] = from[e];
                         }
+                        cp_async_arrive(&bar_raw_q[w]);
                     }
-                    cp_async_commit();
-                    cp_async_wait<0>();
-                    // bf16 rows whose largest value f16 holds with room to spare above and below are converted as
-                    // they are (what f16's subnormals then cut off is below 2^-21 of it), others are scaled to
-                    // [1, 2) first; a negative softmax scale turns q's sign: the scores' factors stay positive
-                    if (!std::is_same<T, __half>::value || a.scale < 0.f)
-                        for (int w = 0; w < n_w; w++)
-#pragma unroll 2
-                            for (int q = 0; q < NI; q++) {
-                                const int rt = cw * 32 + q * RPI + lane / LPR;
-                                uint4 *at = reinterpret_cast<uint4 *>(dst + w * L::q + rt * 128 + (((ch & 7) ^ (rt & 7)) << 4));
-                                uint4 u = *at;
-                                if constexpr (!std::is_same<T, __half>::value) {
-                                    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
-                                    const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
-                                    const uint32_t mb = *reinterpret_cast<const uint32_t *>(&m);
-                                    uint32_t mx = max(mb & 0xffffu, mb >> 16);  // bits of a magnitude: ordered like the magnitudes
-#pragma unroll
-                                    for (int o = 1; o < LPR; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                                    const int e = (int)(mx >> 7) - 127;  // (128: inf or NaN)
-                                    const int eu = mx != 0 && e < 128 && (e < -3 || e > 13) ? min(max(-e, -126), 60) : 0;
-                                    if (ch == 0) reinterpret_cast<int8_t *>(sm + L::crow_off)[odd * kTcRows + w * 128 + rt] = (int8_t)-eu;
-                                    const float f = exp2i(eu);
-                                    const uint32_t v[4] = {u.x, u.y, u.z, u.w};
-                                    uint32_t o[4];
-#pragma unroll
-                                    for (int p = 0; p < 4; p++) o[p] = pack_f16(__uint_as_float(v[p] << 16) * f, __uint_as_float(v[p] & 0xffff0000u) * f);
-                                    u = make_uint4(o[0], o[1], o[2], o[3]);
-                                }
-                                if (a.scale < 0.f) { u.x ^= 0x80008000u; u.y ^= 0x80008000u; u.z ^= 0x80008000u; u.w ^= 0x80008000u; }
-                                *at = u;
-                            }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0)
-                        for (int w = 0; w < n_w; w++) mbar_arrive(&bar_q[w]);
                 }
                 const int rs = n % kTcRaw, cs = n % kTcSlots, g = n >> 1;
                 if (!(ok = attn_wait(&raw_full[rs], (n / kTcRaw) & 1, abort_flag))) break;
