@@ -107,6 +107,8 @@ __device__ __forceinline__ float ex2(float x) {
 constexpr int kKeyTile = 64;    // keys of one stage
 constexpr int kKvStages = 4;
 
+constexpr int kMaxSplits = 128;
+
 // Where a call's split parts go: normalised rows and their log2 weights, [split][row][query head].
 struct AttnParts {
     float *o = nullptr;    // [splits][n_rows * n_q][head_dim]
@@ -468,40 +470,59 @@ __global__ void __launch_bounds__((MW * KW + 1) * 32, MW * KW <= 4 ? 2 : 1)
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = fmaf(p[e], f, v[e]);
         }
-        const float inv = ll > 0.f ? 1.f / ll : 0.f, lw = ll > 0.f ? b + log2f(ll) : -INFINITY;
+        const float inv = ll == 0.f ? 0.f : 1.f / ll, lw = ll == 0.f ? -INFINITY : b + log2f(ll);  // (NaN stays NaN)
 #pragma unroll
         for (int e = 0; e < 8; e++) v[e] *= inv;
         attn_store<T, HD>(a, parts, split, sq.r0 + R / rep, kvh * rep + R % rep, d0, v, lw, vec);
     }
 }
 
-// Joins the split parts of one row and head per warp; rows of no sequence stay as they are.
+// Joins the split parts of one row and head per warp; rows of no sequence stay as they are.  The lanes
+// share out the parts' weights, then each holds four (HD 64: two) dimensions with eight parts' loads in
+// flight: the parts come from L2, and a thread that waited for one after the other took 20 us for 37.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv_attn_join_kernel(const dfb_kv_cache c, const dfb_kv_attn a, const AttnParts parts, bool vec) {
-    constexpr int LPR = HD / 8;  // lanes per row: eight dimensions each
+__global__ void __launch_bounds__(128) kv_attn_join_kernel(const dfb_kv_cache c, const dfb_kv_attn a, const AttnParts parts) {
+    constexpr int E = HD / 32;
     griddep_wait();
     const AttnSeq sq = attn_seq(c, a, blockIdx.y, false, nullptr);
-    const int at = (blockIdx.x * 256 + threadIdx.x) / LPR, d0 = threadIdx.x % LPR * 8;
+    const int at = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (at >= sq.n_rows * a.n_q) return;
     const size_t stride = (size_t)a.n_rows * a.n_q, row = (size_t)sq.r0 * a.n_q + at;
-    float mx = -INFINITY, z = 0.f, v[8] = {};
-    for (int k = 0; k < parts.splits; k++) mx = fmaxf(mx, parts.w[k * stride + row]);
-    if (mx > -INFINITY)
-        for (int k = 0; k < parts.splits; k++) {
-            const float w = parts.w[k * stride + row];
-            if (w == -INFINITY) continue;
-            const float f = ex2(w - mx);
-            z += f;
-            float u[8];
-            load8(parts.o + (k * stride + row) * HD + d0, true, u);
+    float w[kMaxSplits / 32], mx = -INFINITY, z = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = fmaf(u[e], f, v[e]);
+    for (int i = 0; i < kMaxSplits / 32; i++) {
+        w[i] = 32 * i + lane < parts.splits ? parts.w[(32 * i + lane) * stride + row] : -INFINITY;
+        mx = fmaxf(mx, w[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float base = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; i++) {
+        w[i] = ex2(w[i] - base);
+        z += w[i];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    float v[E] = {};
+#pragma unroll
+    for (int i = 0; i < kMaxSplits / 32; i++)
+#pragma unroll 8
+        for (int k = 32 * i; k < min(parts.splits, 32 * i + 32); k++) {
+            const float f = __shfl_sync(0xffffffffu, w[i], k & 31);
+            float u[E];
+            const float *o = parts.o + (k * stride + row) * HD + lane * E;
+            if constexpr (E == 4) *reinterpret_cast<float4 *>(u) = *reinterpret_cast<const float4 *>(o);
+            else *reinterpret_cast<float2 *>(u) = *reinterpret_cast<const float2 *>(o);
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = f == 0.f ? v[e] : fmaf(u[e], f, v[e]);  // (a part without keys is not written)
         }
-    const float inv = z > 0.f ? 1.f / z : 0.f;
+    const float inv = z == 0.f ? 0.f : 1.f / z;  // (NaN stays NaN)
+    const int tok = sq.r0 + at / a.n_q, head = at % a.n_q;
+    T *out = reinterpret_cast<T *>(a.out) + tok * a.out_tok + head * a.out_head + lane * E;
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] *= inv;
-    const AttnParts none;
-    attn_store<T, HD>(a, none, 0, sq.r0 + at / a.n_q, at % a.n_q, d0, v, z > 0.f ? mx + log2f(z) : -INFINITY, vec);
+    for (int e = 0; e < E; e++) out[e] = from_f32<T>(v[e] * inv);
+    if (a.lse && lane == 0) a.lse[row] = z == 0.f ? -INFINITY : (base + log2f(z)) * kLn2;
 }
 
 }  // namespace dfb

@@ -469,9 +469,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     const bool mine = R < it->n_packed;
                     const int t = R / rep, tok = it->r0 + t, head = it->kvh * rep + R - t * rep;
                     const size_t row = (size_t)tok * a.n_q + head, part = (size_t)it->split * a.n_rows * a.n_q + row;
-                    const float inv = l > 0.f ? 1.f / l : 0.f;
+                    const float inv = l == 0.f ? 0.f : 1.f / l;  // (NaN stays NaN)
                     if (half == 0 && mine) {
-                        const float lw = l > 0.f ? M + log2f(l) : -INFINITY;
+                        const float lw = l == 0.f ? -INFINITY : M + log2f(l);
                         if (parts.o) parts.w[part] = lw;
                         else if (a.lse) a.lse[row] = lw * kLn2;
                     }
@@ -486,12 +486,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
 #pragma unroll
-                                for (int e = 0; e < 8; e++) u[e] = l > 0.f ? __float_as_uint(__uint_as_float(o[8 * h + e]) * inv) : 0;
+                                for (int e = 0; e < 8; e++) u[e] = __float_as_uint(__uint_as_float(o[8 * h + e]) * inv);
                                 store_row32(parts.o + part * HD + d0 + 8 * h, 16, u);
                             }
                         } else {
 #pragma unroll
-                            for (int e = 0; e < 16; e++) reinterpret_cast<T *>(u)[e] = from_f32<T>(l > 0.f ? __uint_as_float(o[e]) * inv : 0.f);
+                            for (int e = 0; e < 16; e++) reinterpret_cast<T *>(u)[e] = from_f32<T>(__uint_as_float(o[e]) * inv);
                             store_row32(reinterpret_cast<T *>(a.out) + tok * a.out_tok + head * a.out_head + d0, out_align, u);
                         }
                     }

@@ -1,9 +1,23 @@
 // Log probabilities of given tokens, entropy and top alternatives of logits rows
-// (dfb_token_logprobs).  With m = max x and z = sum exp(x - m):
-//   log p_t = (x_t - m) - log z,   H = log z + sum exp(x - m) (m - x) / z,
-// both terms of H non-negative, so nothing cancels.
+// (dfb_token_logprobs), in one pass over the row.
+//
+// With m = max x, z = sum 2^y and t = sum -y 2^y over y = (x - m) log2(e):
+//   log p_t = (x_t - m) - ln z,   H = ln z + ln 2 t / z,
+// both terms of H non-negative, so nothing cancels.  A thread carries (m, z, t) of its elements and
+// rescales when a batch of them raises m; the parts are joined in a fixed order.  y is held above -200,
+// where 2^y is 0 in f32, so that logits of -inf add 0 to t; a NaN or +inf makes z NaN.
+//
+// Alternatives.  An element's key orders by value, then lower id.  The first batch, spread over the
+// whole row, gives a threshold: the k-th largest of 32 groups' largest keys, no larger than the row's
+// k-th key.  What passes it (some tens of elements; a batch's largest value tells whether it is worth a
+// look) goes to a list in shared memory, whose members' ranks are counted in the end.  A row that
+// overflows the list (ascending logits, say) is gone through again with a threshold that rises.
+//
+// Bound: the row read once from memory.  A row is split over the CTAs of a cluster (joined through
+// distributed shared memory) where rows alone would leave SMs without work.
 #pragma once
 #include <cstdint>
+#include <type_traits>
 
 #include "../../../include/diffuse_b200.h"
 #include "kv_append.cuh"
@@ -11,78 +25,367 @@
 
 namespace dfb {
 
-constexpr int kLpThreads = 512;
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpMaxK = 32, kLpCap = 4096;
+constexpr float kLpLn2 = 0.6931471805599453f, kLpLog2e = 1.4426950408889634f, kLpFloor = -200.f;
 
-// The plain kernel: one block per row, one pass for m, z and the entropy sum, then one pass per
-// alternative (the largest key below the last one; a key orders by value, then lower id).
+struct LpSmem {
+    unsigned long long list[kLpCap];
+    unsigned long long top[kLpMaxK];      // this CTA's k largest keys, in order
+    unsigned long long group[32];
+    float m[kLpWarps], z[kLpWarps], t[kLpWarps];
+    float part[3];                        // this CTA's m, z, t
+    int count, n_top;
+    unsigned long long thr;
+};
+
+__device__ __forceinline__ unsigned long long lp_key(float x, int id) {
+    const uint32_t u = __float_as_uint(x + 0.f);  // (one zero)
+    return (unsigned long long)((u & 0x80000000u) ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - (uint32_t)id);
+}
+__device__ __forceinline__ float lp_value(unsigned long long key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int lp_id(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
+__device__ __forceinline__ float lp_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// max that hands on a NaN
+__device__ __forceinline__ float lp_max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// A word of the same variable in CTA `rank` of the cluster.
+__device__ __forceinline__ float ld_cluster_f32(const float *p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_cluster_s32(const int *p, int rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned long long ld_cluster_u64(const unsigned long long *p, int rank) {
+    unsigned long long v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_shared(p, rank)) : "memory");
+    return v;
+}
+
+struct LpSum {
+    float m = -3.402823466e38f, z = 0.f, t = 0.f;  // (z = 0: nothing but -inf so far)
+    __device__ __forceinline__ void raise(float mn) {  // mn >= m
+        const float y = lp_max_nan((m - mn) * kLpLog2e, kLpFloor), f = lp_ex2(y);
+        t = f * fmaf(-y, z, t);
+        z *= f;
+        m = mn;
+    }
+    __device__ __forceinline__ void join(LpSum o) {
+        if (o.m > m) raise(o.m);
+        else o.raise(m);
+        z += o.z;
+        t += o.t;
+    }
+};
+
+// One batch: NV 16-byte pieces of a thread, as NV * PER values.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logprobs_simple(const dfb_logprob_args a, int32_t *status) {
-    __shared__ float sm[16], sz[16], st[16];
-    __shared__ unsigned long long sk[16];
-    const int i = blockIdx.x, V = a.n_vocab, tid = threadIdx.x;
-    auto flag = [&](int bit) { if (status && tid == 0) atomicOr(status, bit); };
+struct LpBatch {
+    static constexpr int NV = 4, PER = 16 / sizeof(T), N = NV * PER;
+    uint4 raw[NV];
+    __device__ __forceinline__ float at(int i) const {
+        const uint4 &u = raw[i / PER];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const int e = i % PER;
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+        const uint32_t h = w[e / 2];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e & 1 ? h & 0xffff0000u : h << 16);
+        const __half2 p = *reinterpret_cast<const __half2 *>(&h);
+        return e & 1 ? __high2float(p) : __low2float(p);
+    }
+};
+
+// A key above the threshold goes to the list; full: it is counted only.
+__device__ __forceinline__ void lp_push(LpSmem &s, unsigned long long key) {
+    const int at = atomicAdd(&s.count, 1);
+    if (at < kLpCap) s.list[at] = key;
+}
+// The k largest of n keys (n >= 0, all different) to top, in order; every thread of the block takes part.
+__device__ __forceinline__ void lp_rank(const unsigned long long *list, int n, unsigned long long *top, int k) {
+    for (int i = threadIdx.x; i < n; i += kLpThreads) {
+        const unsigned long long key = list[i];
+        int r = 0;
+        for (int j = 0; j < n; j++) r += list[j] > key;
+        if (r < k) top[r] = key;
+    }
+}
+
+// Grid: rows x cluster size; CTA `rank` of a row's cluster takes an equal share of its 16-byte pieces.
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logprob_args a, int32_t *status) {
+    using B = LpBatch<T>;
+    __shared__ LpSmem s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.n_vocab, k = a.top_k;
+    const int rank = (int)cluster_ctarank(), n_cta = (int)(gridDim.x / (unsigned)a.n_rows), i = blockIdx.x / n_cta;
+    auto flag = [&](int bit) { if (status) atomicOr(status, bit); };
     const int row = a.rows ? a.rows[i] : i;
     const bool there = row >= 0 && row < a.n_logits;
-    if (!there) flag(DFB_STAT_TARGET);
     const T *x = reinterpret_cast<const T *>(a.logits) + (size_t)(there ? row : 0) * a.ld;
-    float m = -INFINITY, z = 0.f, t = 0.f;
-    bool bad = !there;
-    auto join = [](float &m, float &z, float &t, float m2, float z2, float t2) {
-        if (m2 == -INFINITY) return;
-        if (m == -INFINITY) { m = m2; z = z2; t = t2; return; }
-        const float mn = fmaxf(m, m2), d1 = fmaxf(m - mn, -1e30f), d2 = fmaxf(m2 - mn, -1e30f), f1 = expf(d1), f2 = expf(d2);
-        t = f1 * (t - z * d1) + f2 * (t2 - z2 * d2);  // sum e^(x - mn) (mn - x)
-        z = f1 * z + f2 * z2;
-        m = mn;
-    };
-    if (there)
-        for (int v = tid; v < V; v += kLpThreads) {
-            const float f = to_f32<T>(x[v]);
-            if (!(f < INFINITY)) bad = true;
-            else join(m, z, t, f, 1.f, 0.f);
-        }
-    bad = __syncthreads_or(bad);
-    for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), z2 = __shfl_xor_sync(0xffffffffu, z, o), t2 = __shfl_xor_sync(0xffffffffu, t, o);
-        join(m, z, t, m2, z2, t2);
-    }
-    if ((tid & 31) == 0) { sm[tid >> 5] = m; sz[tid >> 5] = z; st[tid >> 5] = t; }
-    __syncthreads();
-    m = -INFINITY; z = 0.f; t = 0.f;
-    for (int w = 0; w < kLpThreads / 32; w++) join(m, z, t, sm[w], sz[w], st[w]);
-    if (bad && there) flag(DFB_STAT_LOGITS);
-    const float lz = logf(z);
-    auto lp = [&](float f) { return bad ? NAN : m == -INFINITY ? -INFINITY : (f - m) - lz; };
+    // elements before the first 16-byte boundary and behind the last; pieces of this CTA [v0, v1)
+    const int head = min(V, (int)((16 - reinterpret_cast<uintptr_t>(x) % 16) % 16 / sizeof(T)));
+    const int pieces = (V - head) / B::PER, tail = head + pieces * B::PER;
+    const int v0 = (int)((long long)pieces * rank / n_cta), v1 = (int)((long long)pieces * (rank + 1) / n_cta);
+    const uint4 *body = reinterpret_cast<const uint4 *>(x + head);
+    const int tg = rank == 0 && a.logprob && there ? a.targets[i] : -1;
+    const float xt = tg >= 0 && tg < V ? to_f32<T>(x[tg]) : 0.f;  // (under way beside the row)
     if (tid == 0) {
-        if (a.entropy) a.entropy[i] = bad ? NAN : m == -INFINITY ? 0.f : lz + t / z;
-        if (a.logprob) {
-            const int tg = a.targets[i];
-            if (tg >= V) flag(DFB_STAT_TARGET);
-            a.logprob[i] = tg < 0 ? 0.f : tg >= V ? NAN : lp(to_f32<T>(x[tg]));
+        s.count = 0;
+        s.n_top = 0;
+        s.thr = 0;
+    }
+    __syncthreads();
+    LpSum sum;
+    unsigned long long thr = 0;   // what passes goes to the list
+    float thr_x = -INFINITY;      // its value
+
+    // the pieces of a batch lie a quarter of the range apart
+    const int quarter = ((v1 - v0 + 3) / 4 + kLpThreads - 1) / kLpThreads * kLpThreads;  // in pieces
+    const int rounds = there ? quarter / kLpThreads : 0;
+    auto load = [&](B &b, int r) {
+#pragma unroll
+        for (int u = 0; u < B::NV; u++) {
+            const int o = r * kLpThreads + tid, v = v0 + u * quarter + o;
+            const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+            b.raw[u] = make_uint4(none, none, none, none);
+            if (r < rounds && v < v1) b.raw[u] = __ldcs(body + v);
+        }
+    };
+    auto id_of = [&](int r, int e) { return head + (v0 + e / B::PER * quarter + r * kLpThreads + tid) * B::PER + e % B::PER; };
+    // scalar elements (at most one of each kind a thread): head by the first CTA, tail by the last
+    const bool has_head = there && rank == 0 && tid < head, has_tail = there && rank == n_cta - 1 && tid < V - tail;
+    const float x_head = has_head ? to_f32<T>(x[tid]) : -INFINITY, x_tail = has_tail ? to_f32<T>(x[tail + tid]) : -INFINITY;
+    auto add = [&](const B &b, float bm) {
+        if (bm > sum.m) sum.raise(bm);
+        float z[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < B::N; e++) {
+            const float y = lp_max_nan((b.at(e) - sum.m) * kLpLog2e, kLpFloor), p = lp_ex2(y);
+            z[e & 1] += p;
+            t[e & 1] = fmaf(-y, p, t[e & 1]);
+        }
+        sum.z += z[0] + z[1];
+        sum.t += t[0] + t[1];
+    };
+    auto add1 = [&](float f) {
+        if (f > sum.m) sum.raise(f);
+        const float y = lp_max_nan((f - sum.m) * kLpLog2e, kLpFloor), p = lp_ex2(y);
+        sum.z += p;
+        sum.t = fmaf(-y, p, sum.t);
+    };
+    auto largest = [&](const B &b) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < B::N; e++) m = fmaxf(m, b.at(e));
+        return m;
+    };
+    auto look = [&](const B &b, int r, float bm) {
+        if (bm < thr_x || bm == -INFINITY) return;
+#pragma unroll
+        for (int e = 0; e < B::N; e++) {
+            const float f = b.at(e);
+            if (f >= thr_x && f > -INFINITY) {  // (-inf is no alternative here: see the end)
+                const unsigned long long key = lp_key(f, id_of(r, e));
+                if (key >= thr) lp_push(s, key);
+            }
+        }
+    };
+    auto look1 = [&](float f, int id) {
+        if (f > -INFINITY && lp_key(f, id) >= thr) lp_push(s, lp_key(f, id));
+    };
+    B cur, nxt;
+    load(cur, 0);
+    load(nxt, 1);
+    {
+        const float bm = largest(cur);
+        if (k > 0 && v1 - v0 > kLpCap / B::PER) {
+            // threshold: the k-th of the largest keys of 32 groups of 16 threads
+            unsigned long long key = 0;
+#pragma unroll
+            for (int e = 0; e < B::N; e++)
+                if (cur.at(e) == bm && bm > -INFINITY) {
+                    const unsigned long long c = lp_key(bm, id_of(0, e));
+                    key = c > key ? c : key;
+                }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) {
+                const unsigned long long c = __shfl_xor_sync(0xffffffffu, key, o);
+                key = c > key ? c : key;
+            }
+            if ((lane & 15) == 0) s.group[tid >> 4] = key;
+            __syncthreads();
+            if (warp == 0) {
+                const unsigned long long mine = s.group[lane];
+                int r = 0;
+#pragma unroll
+                for (int j = 0; j < 32; j++) {
+                    const unsigned long long c = s.group[j];
+                    r += c > mine || (c == mine && j < lane);
+                }
+                if (r == k - 1) s.thr = mine;
+            }
+            __syncthreads();
+            thr = s.thr;
+            thr_x = thr ? lp_value(thr) : -INFINITY;
+        }
+        add(cur, bm);
+        if (k > 0) look(cur, 0, bm);
+        if (has_head) {
+            add1(x_head);
+            if (k > 0) look1(x_head, tid);
+        }
+        if (has_tail) {
+            add1(x_tail);
+            if (k > 0) look1(x_tail, tail + tid);
         }
     }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < a.top_k; k++) {
-        unsigned long long best = 0;
-        if (!bad)
-            for (int v = tid; v < V; v += kLpThreads) {
-                const uint32_t u = __float_as_uint(to_f32<T>(x[v]) + 0.f);
-                const unsigned long long key = (unsigned long long)((u & 0x80000000u) ? ~u : u | 0x80000000u) << 32 | (0xffffffffu - v);
-                if (key < last && key > best) best = key;
+    for (int r = 1; r < rounds; r++) {
+        cur = nxt;
+        load(nxt, r + 1);
+        const float bm = largest(cur);
+        add(cur, bm);
+        if (k > 0) look(cur, r, bm);
+    }
+    // ── the block's sums, its k largest keys ──
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        LpSum p;
+        p.m = __shfl_xor_sync(0xffffffffu, sum.m, o);
+        p.z = __shfl_xor_sync(0xffffffffu, sum.z, o);
+        p.t = __shfl_xor_sync(0xffffffffu, sum.t, o);
+        sum.join(p);
+    }
+    if (lane == 0) { s.m[warp] = sum.m; s.z[warp] = sum.z; s.t[warp] = sum.t; }
+    __syncthreads();
+    if (tid == 0) {
+        sum = LpSum();
+        for (int w = 0; w < kLpWarps; w++) {
+            LpSum p;
+            p.m = s.m[w]; p.z = s.z[w]; p.t = s.t[w];
+            sum.join(p);
+        }
+        s.part[0] = sum.m; s.part[1] = sum.z; s.part[2] = sum.t;
+    }
+    if (k > 0) {
+        if (s.count > kLpCap) {
+            // again, two values a thread at a time, the list cut to its k largest whenever the next two might
+            // not fit: the threshold rises to the k-th key so far
+            __syncthreads();
+            if (tid == 0) s.count = 0;
+            __syncthreads();
+            auto cut = [&] {
+                __syncthreads();
+                const int n = s.count;
+                if (n + 2 * kLpThreads > kLpCap) {
+                    lp_rank(s.list, n, s.top, k);
+                    __syncthreads();
+                    if (tid < k) s.list[tid] = s.top[tid];
+                    if (tid == 0) s.count = k;
+                    thr = s.top[k - 1];
+                    thr_x = lp_value(thr);
+                }
+                __syncthreads();
+            };
+            if (has_head) look1(x_head, tid);
+            if (has_tail) look1(x_tail, tail + tid);
+            for (int r = 0; r < rounds; r++) {
+                load(cur, r);
+                for (int e0 = 0; e0 < B::N; e0 += 2) {
+                    cut();
+#pragma unroll
+                    for (int e = 0; e < B::N; e++)
+                        if (e / 2 == e0 / 2) look1(cur.at(e), id_of(r, e));
+                }
             }
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long b2 = __shfl_xor_sync(0xffffffffu, best, o);
-            best = b2 > best ? b2 : best;
         }
         __syncthreads();
-        if ((tid & 31) == 0) sk[tid >> 5] = best;
-        __syncthreads();
-        for (int w = 0; w < kLpThreads / 32; w++) best = sk[w] > best ? sk[w] : best;
-        last = best;
-        if (tid == 0) {
-            const int id = bad ? -1 : (int)(0xffffffffu - (uint32_t)best);
-            a.top_ids[(size_t)i * a.top_k + k] = id;
-            a.top_logprob[(size_t)i * a.top_k + k] = bad ? NAN : lp(to_f32<T>(x[id]));
+        const int n = min(s.count, kLpCap);
+        lp_rank(s.list, n, s.top, k);
+        if (tid == 0) s.n_top = min(n, k);
+    }
+    // ── the cluster's: the first CTA takes the others' ──
+    if (n_cta > 1) {
+        cluster_sync();
+        if (rank == 0) {
+            if (tid == 0) {
+                sum = LpSum();
+                for (int c = 0; c < n_cta; c++) {
+                    LpSum p;
+                    p.m = ld_cluster_f32(&s.part[0], c);
+                    p.z = ld_cluster_f32(&s.part[1], c);
+                    p.t = ld_cluster_f32(&s.part[2], c);
+                    sum.join(p);
+                }
+            }
+            if (k > 0) {
+                if (tid < kLpMaxK * n_cta && tid % kLpMaxK < ld_cluster_s32(&s.n_top, tid / kLpMaxK)) {
+                    const unsigned long long key = ld_cluster_u64(&s.top[tid % kLpMaxK], tid / kLpMaxK);
+                    s.list[tid] = key;
+                } else if (tid < kLpMaxK * n_cta) {
+                    s.list[tid] = 0;  // (no key is 0)
+                }
+            }
+        }
+        cluster_sync();  // the others' shared memory has been read
+        if (rank != 0) return;
+        if (k > 0) {
+            if (tid == 0) s.count = 0;
+            __syncthreads();
+            // the keys that are there, to the front (their order does not matter)
+            unsigned long long key = tid < kLpMaxK * n_cta ? s.list[tid] : 0;
+            __syncthreads();
+            if (key) s.list[atomicAdd(&s.count, 1)] = key;
+            __syncthreads();
+            lp_rank(s.list, s.count, s.top, k);
+            if (tid == 0) s.n_top = min(s.count, k);
+        }
+    } else if (tid == 0) {
+        sum.m = s.part[0]; sum.z = s.part[1]; sum.t = s.part[2];
+    }
+    __syncthreads();
+    if (tid == 0) { s.part[0] = sum.m; s.part[1] = sum.z; s.part[2] = sum.t; }
+    __syncthreads();
+    const float m = s.part[0], z = s.part[1], t = s.part[2];
+    const bool bad = !there || z != z, none = z == 0.f;  // NaN or +inf; nothing but -inf
+    const float lz = logf(z);
+    auto lp = [&](float f) { return bad ? NAN : none ? -INFINITY : (f - m) - lz; };
+    if (tid == 0) {
+        if (!there) flag(DFB_STAT_TARGET);
+        else if (bad) flag(DFB_STAT_LOGITS);
+        if (a.entropy) a.entropy[i] = bad ? NAN : none ? 0.f : fmaf(t / z, kLpLn2, lz);
+        if (a.logprob) {
+            if (tg >= V) flag(DFB_STAT_TARGET);
+            a.logprob[i] = !there ? NAN : tg < 0 ? 0.f : tg >= V ? NAN : lp(xt);
+        }
+    }
+    if (tid < k) {
+        const size_t at = (size_t)i * k + tid;
+        if (bad) {
+            a.top_ids[at] = -1;
+            a.top_logprob[at] = NAN;
+        } else if (tid < s.n_top) {
+            a.top_ids[at] = lp_id(s.top[tid]);
+            a.top_logprob[at] = lp(lp_value(s.top[tid]));
+        } else {
+            // fewer than k logits above -inf: the rest are the lowest ids whose logit is -inf, within the first 2 k
+            int left = tid - s.n_top, id = 0;
+            for (; id < V; id++)
+                if (to_f32<T>(x[id]) == -INFINITY && left-- == 0) break;
+            a.top_ids[at] = id;
+            a.top_logprob[at] = -INFINITY;
         }
     }
 }

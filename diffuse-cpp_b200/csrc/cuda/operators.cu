@@ -141,7 +141,7 @@ AttnPlan attn_plan(const dfb_kv_cache &c, const dfb_kv_attn &a, int n_sm) {
     p.tiles = (int)((packed + p.rows - 1) / p.rows);
     const int64_t base = (int64_t)p.tiles * c.n_kv * c.n_seq, key_tiles = (a.max_keys + kKeyTile - 1) / kKeyTile;
     const int64_t want = (p.rows == kTcRows ? 1 : 2) * n_sm / std::max<int64_t>(base, 1);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, key_tiles / 4, 128}));
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, key_tiles / 4, kMaxSplits}));
     return p;
 }
 size_t attn_ws_bytes(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p) {
@@ -204,8 +204,7 @@ int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float
     }
     if (p.splits > 1) {
         const int64_t per_seq = (int64_t)a.max_rows * a.n_q;
-        CK(launch_k(kv_attn_join_kernel<T, HD>, dim3((unsigned)((per_seq + 256 / (HD / 8) - 1) / (256 / (HD / 8))), c.n_seq), dim3(256), 0, st,
-                    true, c, a, parts, vec));
+        CK(launch_k(kv_attn_join_kernel<T, HD>, dim3((unsigned)((per_seq + 3) / 4), c.n_seq), dim3(128), 0, st, true, c, a, parts));
     }
     return DFB_OK;
 }
@@ -309,11 +308,26 @@ extern "C" int dfb_token_logprobs(const dfb_logprob_args *a, int32_t *status, vo
     int n_sm = 0;
     RET(device_props(g.device(), &n_sm));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // CTAs of a row: as many (up to a cluster of 8) as it takes to give every SM four to work on, but no
+    // fewer than 8 KB of the row to each
+    const int64_t row_bytes = (int64_t)a->n_vocab * type_size(a->type);
+    int n_cta = 1;
+    while (n_cta < 8 && (int64_t)a->n_rows * n_cta < 4 * n_sm && row_bytes / (2 * n_cta) >= 8192) n_cta *= 2;
+    if ((int64_t)a->n_rows * n_cta > INT32_MAX) return set_err(DFB_ERR_UNSUPPORTED, "%d rows", a->n_rows);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(a->n_rows * n_cta));
+    cfg.blockDim = dim3(kLpThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = n_cta;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     switch (a->type) {
-        case T_F32: logprobs_simple<float><<<a->n_rows, kLpThreads, 0, st>>>(*a, status); break;
-        case T_F16: logprobs_simple<__half><<<a->n_rows, kLpThreads, 0, st>>>(*a, status); break;
-        default: logprobs_simple<__nv_bfloat16><<<a->n_rows, kLpThreads, 0, st>>>(*a, status);
+        case T_F32: CK(cudaLaunchKernelEx(&cfg, logprobs_kernel<float>, *a, status)); break;
+        case T_F16: CK(cudaLaunchKernelEx(&cfg, logprobs_kernel<__half>, *a, status)); break;
+        default: CK(cudaLaunchKernelEx(&cfg, logprobs_kernel<__nv_bfloat16>, *a, status));
     }
-    CK(cudaGetLastError());
     return DFB_OK;
 }

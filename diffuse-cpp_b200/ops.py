@@ -64,28 +64,33 @@ def _ck(rc):
         raise DiffuseError(native()[0].dfb_last_error().decode())
 
 
-def _stream(t, stream):
-    return torch.cuda.current_stream(t.device).cuda_stream if stream is None else stream
+def _stream(index, stream):
+    return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream
 
 
-def _ints(name, t, device, n=None):
+# (device indices are compared as integers: a call's checks take a few microseconds, and its kernel may not
+# take more)
+def _ints(name, t, index, n=None):
     """Data pointer of an int32 tensor of the call's GPU (None: a null pointer)."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
+    if t.dtype is not torch.int32 or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be a contiguous int32 tensor on cuda:{index}")
     if n is not None and t.numel() != n:
         raise ValueError(f"{name} has {t.numel()} elements, expected {n}")
     return t.data_ptr()
 
 
-def _rows(name, t, dtype, device, shape):
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {dtype} on {device}")
-    if tuple(t.shape) != shape:
+def _rows(name, t, dtype, index, shape):
+    """(tensor's strides) of rows [n_rows, heads, head_dim]."""
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be {dtype} on cuda:{index}")
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if t.stride(2) != 1:
+    st = t.stride()
+    if st[2] != 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
+    return st
 
 
 class PagedKV:
@@ -103,7 +108,7 @@ class PagedKV:
             if t.dtype != torch.float32 or tuple(t.shape) != tuple(k.shape[:2]) or not t.is_contiguous() or t.device != k.device:
                 raise ValueError(f"scales must be contiguous float32 tensors {tuple(k.shape[:2])} on {k.device}")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.device = k.device
+        self.device, self._index = k.device, k.get_device()
         self.n_pages, self.n_kv, self.page, self.head_dim = k.shape
         self.set_pages(pages)
 
@@ -118,8 +123,9 @@ class PagedKV:
     def set_pages(self, pages):
         if pages.dim() != 2:
             raise ValueError("pages is [n_seq, max_pages]")
-        ptr = _ints("pages", pages, self.device)
-        self.pages = pages
+        ptr = _ints("pages", pages, self._index)
+        self.pages, self._n_seq = pages, pages.shape[0]
+        self._ws = {}  # workspace sizes by the sizes of a call
         self._c = _KvCache(self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(), ptr,
                            self.n_pages, self.n_kv, self.head_dim, self.page, pages.shape[0], pages.shape[1])
         self._ref = C.addressof(self._c)
@@ -133,28 +139,30 @@ def kv_append(cache: PagedKV, k, v, row_off, lens, *, max_rows: int, pos=None, r
     many positions are filled).  max_rows: the most rows of any one sequence.  rope
     [n_positions, head_dim / 2, 2] (f32 cos, sin) rotates k, and q [n_rows, n_q, head_dim] into
     q_out.  See dfb_kv_append for the scales."""
-    d = cache.device
-    if k.dim() != 3 or k.dtype not in _TYPES:
+    d, hd = cache._index, cache.head_dim
+    typ = _TYPES.get(k.dtype)
+    if k.dim() != 3 or typ is None:
         raise ValueError("k is [n_rows, n_kv, head_dim] in f32, f16 or bf16")
-    n, hd = k.shape[0], cache.head_dim
-    _rows("k", k, k.dtype, d, (n, cache.n_kv, hd))
-    _rows("v", v, k.dtype, d, (n, cache.n_kv, hd))
-    r = _KvRows(k.data_ptr(), v.data_ptr(), _TYPES[k.dtype], n, max_rows, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                _ints("row_off", row_off, d, cache._c.n_seq + 1), _ints("lens", lens, d, cache._c.n_seq), _ints("pos", pos, d, n))
+    n = k.shape[0]
+    sk = _rows("k", k, k.dtype, d, (n, cache.n_kv, hd))
+    sv = _rows("v", v, k.dtype, d, (n, cache.n_kv, hd))
+    r = _KvRows(k.data_ptr(), v.data_ptr(), typ, n, max_rows, sk[0], sk[1], sv[0], sv[1], _ints("row_off", row_off, d, cache._n_seq + 1),
+                _ints("lens", lens, d, cache._n_seq), _ints("pos", pos, d, n))
     if rope is not None:
-        if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.device != d or tuple(rope.shape[1:]) != (hd // 2, 2):
-            raise ValueError(f"rope must be a contiguous float32 tensor [n_positions, {hd // 2}, 2] on {d}")
+        if rope.dtype is not torch.float32 or not rope.is_contiguous() or rope.get_device() != d or rope.shape[1:] != (hd // 2, 2):
+            raise ValueError(f"rope must be a contiguous float32 tensor [n_positions, {hd // 2}, 2] on {cache.device}")
         r.rope, r.n_rope = rope.data_ptr(), rope.shape[0]
     if (q is None) != (q_out is None):
         raise ValueError("q and q_out go together")
     if q is not None:
         if q.dim() != 3:
             raise ValueError("q is [n_rows, n_q, head_dim]")
-        _rows("q", q, k.dtype, d, (n, q.shape[1], hd))
-        _rows("q_out", q_out, k.dtype, d, (n, q.shape[1], hd))
-        r.n_q, r.q, r.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
-        r.q_tok, r.q_head, r.q_out_tok, r.q_out_head = q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
-    _ck(_fn("dfb_kv_append")(cache._ref, C.addressof(r), _ints("status", status, d, 1), _stream(k, stream)))
+        n_q = q.shape[1]
+        sq = _rows("q", q, k.dtype, d, (n, n_q, hd))
+        so = _rows("q_out", q_out, k.dtype, d, (n, n_q, hd))
+        r.n_q, r.q, r.q_out = n_q, q.data_ptr(), q_out.data_ptr()
+        r.q_tok, r.q_head, r.q_out_tok, r.q_out_head = sq[0], sq[1], so[0], so[1]
+    _ck(_fn("dfb_kv_append")(cache._ref, C.addressof(r), _ints("status", status, d, 1), _stream(d, stream)))
 
 
 def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: int, scale: float | None = None, vis=None,
@@ -164,29 +172,33 @@ def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: i
     max_rows, max_keys: bounds of any one sequence's rows and keys.  scale None: 1 / sqrt(head_dim).
     workspace: a uint8 tensor of at least kv_attention_workspace(...) bytes (None: allocated here).
     Returns out (and lse [n_rows, n_q], the natural log of the softmax denominator)."""
-    d = cache.device
-    if q.dim() != 3 or q.dtype not in (torch.float16, torch.bfloat16):
+    d = cache._index
+    typ = _TYPES.get(q.dtype)
+    if q.dim() != 3 or typ is None or typ == F32:
         raise ValueError("q is [n_rows, n_q, head_dim] in f16 or bf16")
     n, n_q, hd = q.shape
-    _rows("q", q, q.dtype, d, (n, n_q, cache.head_dim))
+    sq = _rows("q", q, q.dtype, d, (n, n_q, cache.head_dim))
     if out is None:
-        out = torch.empty((n, n_q, hd), dtype=q.dtype, device=d)
+        out = q.new_empty((n, n_q, hd))
+        so = (n_q * hd, hd)
     else:
-        _rows("out", out, q.dtype, d, (n, n_q, hd))
-    lse = torch.empty((n, n_q), dtype=torch.float32, device=d) if return_lse else None
-    a = _KvAttn(q.data_ptr(), out.data_ptr(), _TYPES[q.dtype], n_q, n, max_rows, max_keys,
-                hd**-0.5 if scale is None else scale, q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-                _ints("row_off", row_off, d, cache._c.n_seq + 1), _ints("lens", lens, d, cache._c.n_seq), _ints("vis", vis, d, n),
-                None if lse is None else lse.data_ptr())
-    need = C.c_size_t()
-    _ck(_fn("dfb_kv_attention_workspace")(cache._ref, C.addressof(a), C.addressof(need)))
-    if need.value and workspace is None:
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=d)
-    if workspace is not None and (workspace.device != d or not workspace.is_contiguous()):
-        raise ValueError(f"workspace must be a contiguous tensor on {d}")
+        so = _rows("out", out, q.dtype, d, (n, n_q, hd))
+    lse = q.new_empty((n, n_q), dtype=torch.float32) if return_lse else None
+    a = _KvAttn(q.data_ptr(), out.data_ptr(), typ, n_q, n, max_rows, max_keys, hd**-0.5 if scale is None else scale, sq[0], sq[1],
+                so[0], so[1], _ints("row_off", row_off, d, cache._n_seq + 1), _ints("lens", lens, d, cache._n_seq),
+                _ints("vis", vis, d, n), None if lse is None else lse.data_ptr())
+    if workspace is None:
+        need = cache._ws.get((n_q, n, max_rows, max_keys))
+        if need is None:
+            need = cache._ws[n_q, n, max_rows, max_keys] = kv_attention_workspace(cache, n_q=n_q, n_rows=n, max_rows=max_rows,
+                                                                                  max_keys=max_keys)
+        if need:
+            workspace = q.new_empty((need,), dtype=torch.uint8)
+    elif workspace.get_device() != d or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {cache.device}")
     _ck(_fn("dfb_kv_attention")(cache._ref, C.addressof(a), None if workspace is None else workspace.data_ptr(),
                                 0 if workspace is None else workspace.numel() * workspace.element_size(),
-                                _ints("status", status, d, 1), _stream(q, stream)))
+                                _ints("status", status, d, 1), _stream(d, stream)))
     return (out, lse) if return_lse else out
 
 
@@ -207,16 +219,14 @@ def token_logprobs(logits, targets=None, *, top_k: int = 0, rows=None, status=No
         raise ValueError("logits is a CUDA tensor [n_logits, n_vocab] in f32, f16 or bf16")
     if logits.shape[1] > 1 and logits.stride(1) != 1:
         raise ValueError("logits: the last dimension must be contiguous")
-    d, v = logits.device, logits.shape[1]
+    d, v = logits.get_device(), logits.shape[1]
     n = logits.shape[0] if rows is None else rows.numel()
+    k = max(top_k, 0)
     tp = _ints("targets", targets, d, n)
     # one allocation: logprob, entropy, top_logprob, then the ids
-    buf = torch.empty(n * (2 + 2 * max(top_k, 0)), dtype=torch.float32, device=d)
-    lp, ent = buf[:n], buf[n : 2 * n]
-    top = buf[2 * n : (2 + top_k) * n].view(n, top_k)
-    ids = buf[(2 + top_k) * n :].view(torch.int32).view(n, top_k)
+    lp, ent, top, ids = logits.new_empty((n * (2 + 2 * k),), dtype=torch.float32).split((n, n, n * k, n * k))
+    top, ids = top.view(n, k), ids.view(torch.int32).view(n, k)
     a = _Logprobs(logits.data_ptr(), _TYPES[logits.dtype], v, n, logits.shape[0], logits.stride(0), _ints("rows", rows, d), tp,
-                  lp.data_ptr() if tp else None, ent.data_ptr(), top_k, ids.data_ptr() if top_k else None,
-                  top.data_ptr() if top_k else None)
-    _ck(_fn("dfb_token_logprobs")(C.addressof(a), _ints("status", status, d, 1), _stream(logits, stream)))
+                  lp.data_ptr() if tp else None, ent.data_ptr(), top_k, ids.data_ptr() if k else None, top.data_ptr() if k else None)
+    _ck(_fn("dfb_token_logprobs")(C.addressof(a), _ints("status", status, d, 1), _stream(d, stream)))
     return lp if tp else None, ent, ids, top
