@@ -26,6 +26,7 @@
 #include "../../../include/diffuse_b200.h"
 #include "kv_append.cuh"
 #include "ptx.cuh"
+#include "simd.cuh"
 
 namespace dfb {
 
@@ -97,11 +98,6 @@ __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t w, int half) {
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 constexpr int kKeyTile = 64;    // keys of one stage

@@ -116,11 +116,6 @@ __device__ __forceinline__ void tmem_ld_wait32(float *r) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ void tmem_st1(uint32_t taddr, float v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
@@ -138,19 +133,6 @@ __device__ __forceinline__ bool named_bar_any(uint32_t id, uint32_t n, bool v) {
         : "r"(id), "r"(n), "r"((uint32_t)v)
         : "memory");
     return r != 0;
-}
-// Two f32 operations in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;"
-        : "=l"(d)
-        : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)), "l"(*reinterpret_cast<const uint64_t *>(&c)));
-    return *reinterpret_cast<const float2 *>(&d);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<const uint64_t *>(&a)), "l"(*reinterpret_cast<const uint64_t *>(&b)));
-    return *reinterpret_cast<const float2 *>(&d);
 }
 // The factor of a score is kept above 0, so that a masked score of -inf stays -inf where the softmax
 // scale is 0 or the product of the scales underflows; every score times this is 0 beside an exponent.

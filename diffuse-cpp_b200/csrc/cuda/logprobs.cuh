@@ -22,10 +22,11 @@
 #include "../../../include/diffuse_b200.h"
 #include "kv_append.cuh"
 #include "ptx.cuh"
+#include "simd.cuh"
 
 namespace dfb {
 
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32, kLpMaxK = 32, kLpCap = 4096;
+constexpr int kLpThreads = 256, kLpCtas = 4 /* of an SM */, kLpWarps = kLpThreads / 32, kLpMaxK = 32, kLpCap = 4096;
 constexpr float kLpLn2 = 0.6931471805599453f, kLpLog2e = 1.4426950408889634f, kLpFloor = -200.f;
 
 struct LpSmem {
@@ -35,7 +36,6 @@ struct LpSmem {
     float m[kLpWarps], z[kLpWarps], t[kLpWarps];
     float part[3];                        // this CTA's m, z, t
     int count, n_top;
-    unsigned long long thr;
 };
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int id) {
@@ -47,18 +47,6 @@ __device__ __forceinline__ float lp_value(unsigned long long key) {
     return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ int lp_id(unsigned long long key) { return (int)(0xffffffffu - (uint32_t)key); }
-__device__ __forceinline__ float lp_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// max that hands on a NaN
-__device__ __forceinline__ float lp_max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // A word of the same variable in CTA `rank` of the cluster.
 __device__ __forceinline__ float ld_cluster_f32(const float *p, int rank) {
     float v;
@@ -76,10 +64,21 @@ __device__ __forceinline__ unsigned long long ld_cluster_u64(const unsigned long
     return v;
 }
 
+// Sums relative to 2^b, b = m log2(e) rounded: y = x log2(e) - b is one fused multiply-add.  With
+// d = m log2(e) - b the sum relative to m is z 2^-d, and b's rounding leaves ln z + ln 2 t / z as it is.
+// Beside f32's largest values the products overflow: y comes from x - m there (b = 0 stands for it).
 struct LpSum {
     float m = -3.402823466e38f, z = 0.f, t = 0.f;  // (z = 0: nothing but -inf so far)
+    __device__ __forceinline__ static bool wide(float m) { return fabsf(m) > 1e38f; }
+    __device__ __forceinline__ static float base(float m) { return wide(m) ? 0.f : m * kLpLog2e; }
+    // log2 of what a sum relative to `from` is worth relative to `to` (to >= from)
+    __device__ __forceinline__ static float shift(float from, float to) {
+        if (from == to) return 0.f;
+        if (wide(from) || wide(to)) return max_nan((from - to) * kLpLog2e, kLpFloor);
+        return max_nan(base(from) - base(to), kLpFloor);
+    }
     __device__ __forceinline__ void raise(float mn) {  // mn >= m
-        const float y = lp_max_nan((m - mn) * kLpLog2e, kLpFloor), f = lp_ex2(y);
+        const float y = shift(m, mn), f = ex2(y);
         t = f * fmaf(-y, z, t);
         z *= f;
         m = mn;
@@ -90,12 +89,23 @@ struct LpSum {
         z += o.z;
         t += o.t;
     }
+    __device__ __forceinline__ float log_z() const {  // ln of the sum relative to m
+        const float d = wide(m) ? 0.f : fmaf(m, kLpLog2e, -base(m));
+        return fmaf(-d, kLpLn2, logf(z));
+    }
+    __device__ __forceinline__ float entropy() const { return fmaf(t / z, kLpLn2, logf(z)); }
+    __device__ __forceinline__ void add1(float f) {
+        if (f > m) raise(f);
+        const float y = max_nan(wide(m) ? (f - m) * kLpLog2e : fmaf(f, kLpLog2e, -base(m)), kLpFloor), p = ex2(y);
+        z += p;
+        t = fmaf(-y, p, t);
+    }
 };
 
-// One batch: NV 16-byte pieces of a thread, as NV * PER values.
+// One batch: 16 values of a thread, in NV 16-byte pieces.
 template <typename T>
 struct LpBatch {
-    static constexpr int NV = 4, PER = 16 / sizeof(T), N = NV * PER;
+    static constexpr int PER = 16 / sizeof(T), N = 16, NV = N / PER;
     uint4 raw[NV];
     __device__ __forceinline__ float at(int i) const {
         const uint4 &u = raw[i / PER];
@@ -126,7 +136,7 @@ __device__ __forceinline__ void lp_rank(const unsigned long long *list, int n, u
 
 // Grid: rows x cluster size; CTA `rank` of a row's cluster takes an equal share of its 16-byte pieces.
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logprob_args a, int32_t *status) {
+__global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb_logprob_args a, int32_t *status) {
     using B = LpBatch<T>;
     __shared__ LpSmem s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.n_vocab, k = a.top_k;
@@ -145,23 +155,28 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logpr
     if (tid == 0) {
         s.count = 0;
         s.n_top = 0;
-        s.thr = 0;
     }
     __syncthreads();
     LpSum sum;
     unsigned long long thr = 0;   // what passes goes to the list
     float thr_x = -INFINITY;      // its value
 
-    // the pieces of a batch lie a quarter of the range apart
-    const int quarter = ((v1 - v0 + 3) / 4 + kLpThreads - 1) / kLpThreads * kLpThreads;  // in pieces
+    // the pieces of a batch lie a quarter (16-bit logits: half) of the range apart
+    const int quarter = ((v1 - v0 + B::NV - 1) / B::NV + kLpThreads - 1) / kLpThreads * kLpThreads;  // in pieces
     const int rounds = there ? quarter / kLpThreads : 0;
+    const int full = max(0, (v1 - v0 - (B::NV - 1) * quarter) / kLpThreads);  // rounds that are whole in every part
     auto load = [&](B &b, int r) {
+        const uint4 *p = body + (v0 + r * kLpThreads + tid);
+        if (r < full) {
 #pragma unroll
-        for (int u = 0; u < B::NV; u++) {
-            const int o = r * kLpThreads + tid, v = v0 + u * quarter + o;
-            const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
-            b.raw[u] = make_uint4(none, none, none, none);
-            if (r < rounds && v < v1) b.raw[u] = __ldcs(body + v);
+            for (int u = 0; u < B::NV; u++) b.raw[u] = __ldcs(p + u * quarter);
+        } else if (r < rounds) {
+#pragma unroll
+            for (int u = 0; u < B::NV; u++) {
+                const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+                b.raw[u] = make_uint4(none, none, none, none);
+                if (v0 + u * quarter + r * kLpThreads + tid < v1) b.raw[u] = __ldcs(p + u * quarter);
+            }
         }
     };
     auto id_of = [&](int r, int e) { return head + (v0 + e / B::PER * quarter + r * kLpThreads + tid) * B::PER + e % B::PER; };
@@ -170,94 +185,132 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logpr
     const float x_head = has_head ? to_f32<T>(x[tid]) : -INFINITY, x_tail = has_tail ? to_f32<T>(x[tail + tid]) : -INFINITY;
     auto add = [&](const B &b, float bm) {
         if (bm > sum.m) sum.raise(bm);
-        float z[2] = {0.f, 0.f}, t[2] = {0.f, 0.f};
+        if (LpSum::wide(sum.m)) {
+#pragma unroll 1
+            for (int e = 0; e < B::N; e++) {
+                float f = 0.f;
 #pragma unroll
-        for (int e = 0; e < B::N; e++) {
-            const float y = lp_max_nan((b.at(e) - sum.m) * kLpLog2e, kLpFloor), p = lp_ex2(y);
-            z[e & 1] += p;
-            t[e & 1] = fmaf(-y, p, t[e & 1]);
+                for (int c = 0; c < B::N; c++) f = c == e ? b.at(c) : f;
+                sum.add1(f);
+            }
+            return;
         }
-        sum.z += z[0] + z[1];
-        sum.t += t[0] + t[1];
-    };
-    auto add1 = [&](float f) {
-        if (f > sum.m) sum.raise(f);
-        const float y = lp_max_nan((f - sum.m) * kLpLog2e, kLpFloor), p = lp_ex2(y);
-        sum.z += p;
-        sum.t = fmaf(-y, p, sum.t);
+        const float nb = -LpSum::base(sum.m);
+        float2 z = make_float2(0.f, 0.f), t = z;  // t: of y 2^y
+#pragma unroll
+        for (int e = 0; e < B::N; e += 2) {
+            float2 y = fma2(make_float2(b.at(e), b.at(e + 1)), make_float2(kLpLog2e, kLpLog2e), make_float2(nb, nb));
+            y = make_float2(max_nan(y.x, kLpFloor), max_nan(y.y, kLpFloor));
+            const float2 p = make_float2(ex2(y.x), ex2(y.y));
+            z = add2(z, p);
+            t = fma2(y, p, t);
+        }
+        sum.z += z.x + z.y;
+        sum.t -= t.x + t.y;
     };
     auto largest = [&](const B &b) {
-        float m = -INFINITY;
+        float m = b.at(0);
 #pragma unroll
-        for (int e = 0; e < B::N; e++) m = fmaxf(m, b.at(e));
-        return m;
+        for (int e = 1; e + 1 < B::N; e += 2) m = max3(m, b.at(e), b.at(e + 1));
+        return fmaxf(m, b.at(B::N - 1));
     };
     auto look = [&](const B &b, int r, float bm) {
         if (bm < thr_x || bm == -INFINITY) return;
+        const float least = fmaxf(thr_x, -3.402823466e38f);  // (-inf is no alternative here: see the end)
+        uint32_t pass = 0;
 #pragma unroll
-        for (int e = 0; e < B::N; e++) {
-            const float f = b.at(e);
-            if (f >= thr_x && f > -INFINITY) {  // (-inf is no alternative here: see the end)
-                const unsigned long long key = lp_key(f, id_of(r, e));
-                if (key >= thr) lp_push(s, key);
-            }
+        for (int e = 0; e < B::N; e++) pass |= b.at(e) >= least ? 1u << e : 0u;
+        while (pass) {
+            const int e = __ffs(pass) - 1;
+            pass &= pass - 1;
+            float f = b.at(0);
+#pragma unroll
+            for (int c = 1; c < B::N; c++) f = c == e ? b.at(c) : f;
+            const unsigned long long key = lp_key(f, id_of(r, e));
+            if (key >= thr) lp_push(s, key);
         }
     };
     auto look1 = [&](float f, int id) {
         if (f > -INFINITY && lp_key(f, id) >= thr) lp_push(s, lp_key(f, id));
     };
+    // cuts the list to its k largest and takes the k-th for the threshold
+    auto tighten = [&] {
+        __syncthreads();
+        const int n = s.count;
+        __syncthreads();  // (no one adds to it before all have read it)
+        if (n < k || n > kLpCap) return;
+        lp_rank(s.list, n, s.top, k);
+        __syncthreads();
+        if (tid < k) s.list[tid] = s.top[tid];
+        if (tid == 0) s.count = k;
+        thr = s.top[k - 1];
+        thr_x = lp_value(thr);
+        __syncthreads();
+    };
     B cur, nxt;
     load(cur, 0);
     load(nxt, 1);
-    {
+    if (rounds > 0) {
         const float bm = largest(cur);
-        if (k > 0 && v1 - v0 > kLpCap / B::PER) {
-            // threshold: the k-th of the largest keys of 32 groups of 16 threads
-            unsigned long long key = 0;
+        // the 32 largest keys of groups of 8 threads: their k-th is the first threshold, the largest value
+        // the m that all threads begin with (with an own one each, some lane of a warp rescales in nearly
+        // every batch)
+        unsigned long long key = 0;
 #pragma unroll
-            for (int e = 0; e < B::N; e++)
-                if (cur.at(e) == bm && bm > -INFINITY) {
-                    const unsigned long long c = lp_key(bm, id_of(0, e));
-                    key = c > key ? c : key;
-                }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) {
-                const unsigned long long c = __shfl_xor_sync(0xffffffffu, key, o);
+        for (int e = 0; e < B::N; e++)
+            if (cur.at(e) == bm && bm > -INFINITY) {
+                const unsigned long long c = lp_key(bm, id_of(0, e));
                 key = c > key ? c : key;
             }
-            if ((lane & 15) == 0) s.group[tid >> 4] = key;
-            __syncthreads();
-            if (warp == 0) {
-                const unsigned long long mine = s.group[lane];
-                int r = 0;
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const unsigned long long c = s.group[j];
-                    r += c > mine || (c == mine && j < lane);
-                }
-                if (r == k - 1) s.thr = mine;
-            }
-            __syncthreads();
-            thr = s.thr;
+        for (int o = 4; o > 0; o >>= 1) {
+            const unsigned long long c = __shfl_xor_sync(0xffffffffu, key, o);
+            key = c > key ? c : key;
+        }
+        if ((lane & 7) == 0) s.group[tid >> 3] = key;
+        __syncthreads();
+        const unsigned long long mine = s.group[lane];  // every warp finds the same
+        int r = 0;
+#pragma unroll
+        for (int j = 0; j < 32; j++) {
+            const unsigned long long c = s.group[j];
+            r += c > mine || (c == mine && j < lane);
+        }
+        const unsigned first = __ballot_sync(0xffffffffu, r == 0), kth = __ballot_sync(0xffffffffu, r == k - 1);
+        const unsigned long long best = __shfl_sync(0xffffffffu, mine, __ffs(first) - 1);
+        if (best) sum.m = lp_value(best);
+        if (k > 0 && v1 - v0 > kLpCap / B::PER) {
+            thr = __shfl_sync(0xffffffffu, mine, __ffs(kth) - 1);
             thr_x = thr ? lp_value(thr) : -INFINITY;
         }
         add(cur, bm);
         if (k > 0) look(cur, 0, bm);
-        if (has_head) {
-            add1(x_head);
-            if (k > 0) look1(x_head, tid);
-        }
-        if (has_tail) {
-            add1(x_tail);
-            if (k > 0) look1(x_tail, tail + tid);
-        }
     }
-    for (int r = 1; r < rounds; r++) {
-        cur = nxt;
-        load(nxt, r + 1);
-        const float bm = largest(cur);
-        add(cur, bm);
-        if (k > 0) look(cur, r, bm);
+    if (has_head) {
+        sum.add1(x_head);
+        if (k > 0) look1(x_head, tid);
+    }
+    if (has_tail) {
+        sum.add1(x_tail);
+        if (k > 0) look1(x_tail, tail + tid);
+    }
+    // a threshold from n of the row's elements lets some k (row / n - 1) more pass: it is taken again after
+    // 1, 4, 13, ... batches (taken once, from groups, 2048 rows of 152064 with k = 20 spent most of their 282 us
+    // on what it let pass)
+    int again = 1;
+    auto batch = [&](const B &b, B &spare, int r) {
+        load(spare, r + 1);
+        if (k > 0 && r == again) {
+            tighten();
+            again = 3 * again + 1;
+        }
+        const float bm = largest(b);
+        add(b, bm);
+        if (k > 0) look(b, r, bm);
+    };
+    for (int r = 1; r < rounds; r += 2) {
+        batch(nxt, cur, r);
+        if (r + 1 < rounds) batch(cur, nxt, r + 1);
     }
     // ── the block's sums, its k largest keys ──
 #pragma unroll
@@ -270,14 +323,18 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logpr
     }
     if (lane == 0) { s.m[warp] = sum.m; s.z[warp] = sum.z; s.t[warp] = sum.t; }
     __syncthreads();
-    if (tid == 0) {
+    if (warp == 0) {
         sum = LpSum();
-        for (int w = 0; w < kLpWarps; w++) {
+        if (lane < kLpWarps) { sum.m = s.m[lane]; sum.z = s.z[lane]; sum.t = s.t[lane]; }
+#pragma unroll
+        for (int o = kLpWarps / 2; o > 0; o >>= 1) {
             LpSum p;
-            p.m = s.m[w]; p.z = s.z[w]; p.t = s.t[w];
+            p.m = __shfl_xor_sync(0xffffffffu, sum.m, o);
+            p.z = __shfl_xor_sync(0xffffffffu, sum.z, o);
+            p.t = __shfl_xor_sync(0xffffffffu, sum.t, o);
             sum.join(p);
         }
-        s.part[0] = sum.m; s.part[1] = sum.z; s.part[2] = sum.t;
+        if (lane == 0) { s.part[0] = sum.m; s.part[1] = sum.z; s.part[2] = sum.t; }
     }
     if (k > 0) {
         if (s.count > kLpCap) {
@@ -288,16 +345,8 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logpr
             __syncthreads();
             auto cut = [&] {
                 __syncthreads();
-                const int n = s.count;
-                if (n + 2 * kLpThreads > kLpCap) {
-                    lp_rank(s.list, n, s.top, k);
-                    __syncthreads();
-                    if (tid < k) s.list[tid] = s.top[tid];
-                    if (tid == 0) s.count = k;
-                    thr = s.top[k - 1];
-                    thr_x = lp_value(thr);
-                }
-                __syncthreads();
+                if (s.count + 2 * kLpThreads > kLpCap) tighten();
+                else __syncthreads();
             };
             if (has_head) look1(x_head, tid);
             if (has_tail) look1(x_tail, tail + tid);
@@ -358,14 +407,14 @@ __global__ void __launch_bounds__(kLpThreads, 2) logprobs_kernel(const dfb_logpr
     __syncthreads();
     if (tid == 0) { s.part[0] = sum.m; s.part[1] = sum.z; s.part[2] = sum.t; }
     __syncthreads();
-    const float m = s.part[0], z = s.part[1], t = s.part[2];
+    sum.m = s.part[0]; sum.z = s.part[1]; sum.t = s.part[2];
+    const float m = sum.m, z = sum.z, lz = sum.log_z();
     const bool bad = !there || z != z, none = z == 0.f;  // NaN or +inf; nothing but -inf
-    const float lz = logf(z);
-    auto lp = [&](float f) { return bad ? NAN : none ? -INFINITY : (f - m) - lz; };
+        auto lp = [&](float f) { return bad ? NAN : none ? -INFINITY : (f - m) - lz; };
     if (tid == 0) {
         if (!there) flag(DFB_STAT_TARGET);
         else if (bad) flag(DFB_STAT_LOGITS);
-        if (a.entropy) a.entropy[i] = bad ? NAN : none ? 0.f : fmaf(t / z, kLpLn2, lz);
+        if (a.entropy) a.entropy[i] = bad ? NAN : none ? 0.f : sum.entropy();
         if (a.logprob) {
             if (tg >= V) flag(DFB_STAT_TARGET);
             a.logprob[i] = !there ? NAN : tg < 0 ? 0.f : tg >= V ? NAN : lp(xt);

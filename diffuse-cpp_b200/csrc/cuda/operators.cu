@@ -308,11 +308,12 @@ extern "C" int dfb_token_logprobs(const dfb_logprob_args *a, int32_t *status, vo
     int n_sm = 0;
     RET(device_props(g.device(), &n_sm));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // CTAs of a row: as many (up to a cluster of 8) as it takes to give every SM four to work on, but no
-    // fewer than 8 KB of the row to each
+    // CTAs of a row (a cluster of up to 8): as many as still run all at once, with 8 KB of the
+    // row to each at least.  More of them would share out the memory's bandwidth better, but each has some
+    // 5 us of its own (first batch, threshold, joining): 256 rows of 126464 took 54 us with four.
     const int64_t row_bytes = (int64_t)a->n_vocab * type_size(a->type);
     int n_cta = 1;
-    while (n_cta < 8 && (int64_t)a->n_rows * n_cta < 4 * n_sm && row_bytes / (2 * n_cta) >= 8192) n_cta *= 2;
+    while (n_cta < 8 && (int64_t)a->n_rows * n_cta * 2 <= kLpCtas * n_sm && row_bytes / (2 * n_cta) >= 8192) n_cta *= 2;
     if ((int64_t)a->n_rows * n_cta > INT32_MAX) return set_err(DFB_ERR_UNSUPPORTED, "%d rows", a->n_rows);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a->n_rows * n_cta));
