@@ -82,6 +82,15 @@ __device__ __forceinline__ float rot_odd(float x, float c, float y, float s, flo
     return __uint_as_float(u | 1u);
 }
 
+// x c + y s within 1.5 units in the last place of it (the rounding error of one product is added back).
+__device__ __forceinline__ float rot_near(float x, float c, float y, float s) {
+    const float p = __fmul_rn(y, s), e = __fmaf_rn(y, s, -p);
+    const float f = __fmaf_rn(x, c, p);
+    return e == 0.f ? f : __fadd_rn(f, e);  // (keeps the sign of a zero)
+}
+// A value that rot_near gives lies within this of the exact one, relative to it (four times the bound).
+constexpr float kRotTol = 4.76837158203125e-07f;  // 2^-21
+
 // Smallest e >= -64 with amax <= 448 * 2^e = 0.875 * 2^(9 + e).
 __device__ __forceinline__ int need_exp(float amax) {
     const uint32_t u = __float_as_uint(amax);
@@ -111,21 +120,34 @@ __device__ __forceinline__ int lower_bound(const int32_t *pos, int lo, int hi, i
     return lo;
 }
 
-constexpr int kAppendThreads = 256;
+// The codes of eight values.
+__device__ __forceinline__ uint2 encode8(const float *v, float inv) {
+    uint2 w;
+    w.x = e4m3_pair(v[0] * inv, v[1] * inv) | e4m3_pair(v[2] * inv, v[3] * inv) << 16;
+    w.y = e4m3_pair(v[4] * inv, v[5] * inv) | e4m3_pair(v[6] * inv, v[7] * inv) << 16;
+    return w;
+}
 
 // One block: the rows that fall into one page of one sequence (the blockIdx.x-th touched page of
-// sequence blockIdx.z), for one head: K heads, then V heads, then query heads (blockIdx.y).  An
-// item is eight values and their rotation partners; a thread holds its items in registers
-// between the maximum and the conversion, so the rows are read once.
-template <typename T, int HD, int ITEMS>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, bool vec,
-                                                                   int32_t *status) {
+// sequence blockIdx.z), for `heads` K heads, V heads or query heads in turn (blockIdx.y).  An item is
+// eight values and their rotation partners; a thread holds its items' cos and sin for all the heads
+// and its values between the maximum and the conversion, so rows are read once and the table's rows
+// once for a group of heads.
+//
+// Bound: memory (rows in, codes out), if the rotation is cheap: rot_odd's sixteen instructions a value
+// took 520 us for 32768 rows of 32 + 32 + 32 heads.  rot_near's four decide every code but those whose
+// value lies within kRotTol of a border of two codes (one in 10^5), and the scale unless the maximum
+// lies that near to 448 * 2^e; those are worked out again with rot_odd.
+template <typename T, int HD, int ITEMS, int kAppendThreads>
+__global__ void __launch_bounds__(kAppendThreads, 512 / kAppendThreads) kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, int heads, bool vec,
+                                                                      int32_t *status) {
     constexpr int IPR = HD / 16;  // items per row
-    __shared__ float red[kAppendThreads / 32];
+    __shared__ float red[2][kAppendThreads / 32];
     __shared__ uint32_t written[4];
     const int s = blockIdx.z, P = c.page, tid = threadIdx.x;
-    const int sec = (int)blockIdx.y < c.n_kv ? 0 : (int)blockIdx.y < 2 * c.n_kv ? 1 : 2;
-    const int head = blockIdx.y - (sec == 0 ? 0 : sec == 1 ? c.n_kv : 2 * c.n_kv);
+    const int groups = (c.n_kv + heads - 1) / heads;  // blocks of the K heads
+    const int sec = (int)blockIdx.y < groups ? 0 : (int)blockIdx.y < 2 * groups ? 1 : 2;
+    const int head0 = (blockIdx.y - (sec == 0 ? 0 : sec == 1 ? groups : 2 * groups)) * heads, head1 = min(head0 + heads, sec == 2 ? r.n_q : c.n_kv);
     auto flag = [&](int bit) { if (status) atomicOr(status, bit); };
     const bool reporter = blockIdx.x == 0 && blockIdx.y == 0;  // one block per sequence reports on its rows
     // the sequence's rows
@@ -134,7 +156,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const dfb_kv_
     if (a < 0 || b < a || b > r.n_rows || b - a > r.max_rows) {
         if (reporter && tid == 0) flag(DFB_STAT_ROWS);
         a = min(max(a, 0), r.n_rows);
-        b = min(min(max(b, a), r.n_rows), a + r.max_rows);
+        b = min(max(b, a), r.n_rows);
+        b = a + min(b - a, r.max_rows);
     }
     if (a == b) return;
     const int cap = c.max_pages * P, limit = r.rope ? min(cap, r.n_rope) : cap;
@@ -143,7 +166,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const dfb_kv_
         return;
     }
     // positions of the rows: first + (row - a), or pos[row]
-    const int first = r.pos ? r.pos[a] : len, last = r.pos ? r.pos[b - 1] : len + (b - a - 1);
+    const int first = r.pos ? r.pos[a] : len;
+    const long long last = r.pos ? r.pos[b - 1] : (long long)len + (b - a - 1);
     if (reporter && (first < 0 || last >= limit) && tid == 0) flag(DFB_STAT_POSITION);
     if (reporter && r.pos)
         for (int i = a + 1 + tid; i < b; i += kAppendThreads)
@@ -172,114 +196,172 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const dfb_kv_
         const bool ok = p >= p0 && p < p0 + P && p < limit && !(r.pos && row > a && r.pos[row - 1] >= p);
         return ok ? p - p0 : -1;
     };
-    const T *src = reinterpret_cast<const T *>(sec == 0 ? r.k : sec == 1 ? r.v : r.q);
-    const int64_t tok = sec == 0 ? r.k_tok : sec == 1 ? r.v_tok : r.q_tok;
-    src += head * (sec == 0 ? r.k_head : sec == 1 ? r.v_head : r.q_head);
+    const int64_t tok = sec == 0 ? r.k_tok : sec == 1 ? r.v_tok : r.q_tok, head_st = sec == 0 ? r.k_head : sec == 1 ? r.v_head : r.q_head;
+    const T *src0 = reinterpret_cast<const T *>(sec == 0 ? r.k : sec == 1 ? r.v : r.q);
     const bool rotate = r.rope && sec != 1;
 
     if (tid < 4) written[tid] = 0;
     __syncthreads();
-    float x[ITEMS][16], amax = 0.f;
     int slot[ITEMS];
-    bool bad = false;
+    float4 cs[ITEMS][4];
+    const T *src[ITEMS];
 #pragma unroll
     for (int j = 0; j < ITEMS; j++) {
         const int it = tid + j * kAppendThreads, row = lo + it / IPR, i = (it % IPR) * 8;
         slot[j] = row < hi ? slot_of(row) : -1;
+        src[j] = src0 + row * tok + i;
         if (slot[j] < 0) continue;
-        float u[8], w[8];
-        load8(src + row * tok + i, vec, u);
-        load8(src + row * tok + i + HD / 2, vec, w);
-        if (rotate) {
-            const float4 *cs = reinterpret_cast<const float4 *>(r.rope + ((size_t)(p0 + slot[j]) * (HD / 2) + i) * 2);
-            float nu[8], nw[8];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float4 t = cs[e];
-                float x0 = rot_odd(u[2 * e], t.x, w[2 * e], -t.y, nu[2 * e]), x1 = rot_odd(u[2 * e], t.y, w[2 * e], t.x, nw[2 * e]);
-                u[2 * e] = x0; w[2 * e] = x1;
-                x0 = rot_odd(u[2 * e + 1], t.z, w[2 * e + 1], -t.w, nu[2 * e + 1]);
-                x1 = rot_odd(u[2 * e + 1], t.w, w[2 * e + 1], t.z, nw[2 * e + 1]);
-                u[2 * e + 1] = x0; w[2 * e + 1] = x1;
-            }
-            if (sec == 2 && sizeof(T) == 4) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) { u[e] = nu[e]; w[e] = nw[e]; }
-            }
-        }
-        if (sec == 2) {
-            T *dst = reinterpret_cast<T *>(r.q_out) + row * r.q_out_tok + head * r.q_out_head + i;
-            store8(dst, vec, u);
-            store8(dst + HD / 2, vec, w);
-            continue;
-        }
         if (i == 0) atomicOr(&written[slot[j] >> 5], 1u << (slot[j] & 31));
+        if (rotate) {
+            const float4 *t = reinterpret_cast<const float4 *>(r.rope + ((size_t)(p0 + slot[j]) * (HD / 2) + i) * 2);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[j][e] = u[e];
-            x[j][8 + e] = w[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const float m = fabsf(x[j][e]);
-            if (m < INFINITY) amax = fmaxf(amax, m);
-            else {
-                bad = true;
-                if (m != m) x[j][e] = 0.f;
-            }
+            for (int e = 0; e < 4; e++) cs[j][e] = __ldg(t + e);
         }
     }
-    if (sec == 2) return;
-    if (bad) flag(DFB_STAT_NONFINITE);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if ((tid & 31) == 0) red[tid >> 5] = amax;
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; w++) amax = fmaxf(amax, red[w]);
-
-    const size_t blk = (size_t)pid * c.n_kv + head;
-    float *scale = (sec == 0 ? c.k_scale : c.v_scale) + blk;
-    uint8_t *codes = reinterpret_cast<uint8_t *>(sec == 0 ? c.k : c.v) + blk * P * HD;
-    int e = need_exp(amax);
     const int kept = min(max(len - p0, 0), P);  // filled positions of the page; those written now do not survive
     bool survive = false;
     for (int t = 0; t < kept; t += 32) {
         const uint32_t all = kept - t >= 32 ? 0xffffffffu : (1u << (kept - t)) - 1;
         survive |= (all & ~written[t >> 5]) != 0;
     }
-    if (survive) {
-        const int old = scale_exp(*scale);
-        if (old >= e) e = old;
-        else {  // grown: re-round the kept codes
-            const float f = exp2i(max(old - e, -126));
-            for (int it = tid; it < kept * (HD / 4); it += kAppendThreads) {
-                const int t = it / (HD / 4);
-                if (written[t >> 5] >> (t & 31) & 1) continue;
-                uint32_t *w = reinterpret_cast<uint32_t *>(codes + t * HD) + it % (HD / 4);
-                const uint32_t v = *w;
-                *w = e4m3_pair(e4m3_value(v & 255) * f, e4m3_value(v >> 8 & 255) * f) |
-                     e4m3_pair(e4m3_value(v >> 16 & 255) * f, e4m3_value(v >> 24) * f) << 16;
+    // item j of a head: its 16 values, rotated within kRotTol, or (exact) rounded to odd
+    auto item = [&](int j, int head, bool exact, float (&x)[16]) {
+        float u[8], w[8];
+        load8(src[j] + head * head_st, vec, u);
+        load8(src[j] + head * head_st + HD / 2, vec, w);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float cc = e & 1 ? cs[j][e / 2].z : cs[j][e / 2].x, ss = e & 1 ? cs[j][e / 2].w : cs[j][e / 2].y;
+            float n;
+            x[e] = !rotate ? u[e] : exact ? rot_odd(u[e], cc, w[e], -ss, n) : rot_near(u[e], cc, w[e], -ss);
+            x[8 + e] = !rotate ? w[e] : exact ? rot_odd(u[e], ss, w[e], cc, n) : rot_near(u[e], ss, w[e], cc);
+        }
+    };
+    // finite values only, and their maximum
+    auto clean = [&](float (&x)[16], float &amax, bool &bad) {
+        float m = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e++) m = fmaxf(m, fabsf(x[e]));
+        bool all = m < INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; e++) all = all && x[e] == x[e];
+        if (!all) {
+            bad = true;
+            m = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                if (x[e] != x[e]) x[e] = 0.f;
+                if (fabsf(x[e]) < INFINITY) m = fmaxf(m, fabsf(x[e]));
             }
         }
+        amax = fmaxf(amax, m);
+    };
+    auto block_max = [&](float v, int buf) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if ((tid & 31) == 0) red[buf][tid >> 5] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kAppendThreads / 32; w++) v = fmaxf(v, red[buf][w]);
+        return v;
+    };
+    if (sec == 2) {
+        for (int head = head0; head < head1; head++)
+#pragma unroll
+            for (int j = 0; j < ITEMS; j++) {
+                if (slot[j] < 0) continue;
+                const int it = tid + j * kAppendThreads, row = lo + it / IPR, i = (it % IPR) * 8;
+                float x[16];
+                if constexpr (sizeof(T) == 4) {  // f32 rows: the nearest f32 of the exact value
+                    float u[8], w[8];
+                    load8(src[j] + head * head_st, vec, u);
+                    load8(src[j] + head * head_st + HD / 2, vec, w);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float cc = e & 1 ? cs[j][e / 2].z : cs[j][e / 2].x, ss = e & 1 ? cs[j][e / 2].w : cs[j][e / 2].y;
+                        x[e] = u[e];
+                        x[8 + e] = w[e];
+                        if (rotate) {
+                            rot_odd(u[e], cc, w[e], -ss, x[e]);
+                            rot_odd(u[e], ss, w[e], cc, x[8 + e]);
+                        }
+                    }
+                } else {
+                    item(j, head, false, x);
+                }
+                T *dst = reinterpret_cast<T *>(r.q_out) + row * r.q_out_tok + head * r.q_out_head + i;
+                store8(dst, vec, reinterpret_cast<float(&)[8]>(x[0]));
+                store8(dst + HD / 2, vec, reinterpret_cast<float(&)[8]>(x[8]));
+            }
+        return;
     }
-    __syncthreads();  // every thread has read the old scale
-    if (tid == 0) *scale = exp2i(e);
-    const float inv = exp2i(-e);
+    bool bad = false;
+    for (int head = head0; head < head1; head++) {
+        const size_t blk = (size_t)pid * c.n_kv + head;
+        float *scale = (sec == 0 ? c.k_scale : c.v_scale) + blk;
+        uint8_t *codes = reinterpret_cast<uint8_t *>(sec == 0 ? c.k : c.v) + blk * P * HD;
+        const int old = survive ? scale_exp(*scale) : 0;  // (every thread has it before block_max lets one write)
+        float x[ITEMS][16], amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < ITEMS; j++) {
-        if (slot[j] < 0) continue;
-        const int i = ((tid + j * kAppendThreads) % IPR) * 8;
-        uint8_t *dst = codes + slot[j] * HD + i;
+        for (int j = 0; j < ITEMS; j++) {
+            if (slot[j] < 0) continue;
+            item(j, head, false, x[j]);
+            clean(x[j], amax, bad);
+        }
+        amax = block_max(amax, head & 1);
+        if (rotate && need_exp(amax * (1.f - kRotTol)) != need_exp(amax * (1.f + kRotTol))) {  // (the same for the whole block)
+            amax = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const float *v = &x[j][8 * h];
-            uint2 w;
-            w.x = e4m3_pair(v[0] * inv, v[1] * inv) | e4m3_pair(v[2] * inv, v[3] * inv) << 16;
-            w.y = e4m3_pair(v[4] * inv, v[5] * inv) | e4m3_pair(v[6] * inv, v[7] * inv) << 16;
-            *reinterpret_cast<uint2 *>(dst + h * (HD / 2)) = w;
+            for (int j = 0; j < ITEMS; j++) {
+                if (slot[j] < 0) continue;
+                float y[16];
+                item(j, head, true, y);
+                clean(y, amax, bad);
+            }
+            __syncthreads();
+            amax = block_max(amax, head & 1);
+            __syncthreads();
+        }
+        int e = need_exp(amax);
+        if (survive) {
+            if (old >= e) e = old;
+            else {  // grown: re-round the kept codes
+                const float f = exp2i(max(old - e, -126));
+                for (int it = tid; it < kept * (HD / 4); it += kAppendThreads) {
+                    const int t = it / (HD / 4);
+                    if (written[t >> 5] >> (t & 31) & 1) continue;
+                    uint32_t *w = reinterpret_cast<uint32_t *>(codes + t * HD) + it % (HD / 4);
+                    const uint32_t v = *w;
+                    *w = e4m3_pair(e4m3_value(v & 255) * f, e4m3_value(v >> 8 & 255) * f) |
+                         e4m3_pair(e4m3_value(v >> 16 & 255) * f, e4m3_value(v >> 24) * f) << 16;
+                }
+            }
+        }
+        if (tid == 0) *scale = exp2i(e);
+        const float inv = exp2i(-e);
+#pragma unroll
+        for (int j = 0; j < ITEMS; j++) {
+            if (slot[j] < 0) continue;
+            uint8_t *dst = codes + slot[j] * HD + ((tid + j * kAppendThreads) % IPR) * 8;
+            uint2 w0 = encode8(&x[j][0], inv), w1 = encode8(&x[j][8], inv);
+            if (rotate) {
+                const float up = inv * (1.f + kRotTol), down = inv * (1.f - kRotTol);
+                const uint2 a0 = encode8(&x[j][0], up), a1 = encode8(&x[j][8], up), b0 = encode8(&x[j][0], down), b1 = encode8(&x[j][8], down);
+                if (a0.x != b0.x || a0.y != b0.y || a1.x != b1.x || a1.y != b1.y) {
+                    float y[16], m = 0.f;
+                    bool ignored = false;
+                    item(j, head, true, y);
+                    clean(y, m, ignored);
+                    w0 = encode8(&y[0], inv);
+                    w1 = encode8(&y[8], inv);
+                }
+            }
+            *reinterpret_cast<uint2 *>(dst) = w0;
+            *reinterpret_cast<uint2 *>(dst + HD / 2) = w1;
         }
     }
+    if (bad) flag(DFB_STAT_NONFINITE);
 }
 
 }  // namespace dfb

@@ -96,11 +96,18 @@ bool vec_ok(const void *p, int type, int64_t tok, int64_t head) {
 }
 
 template <typename T, int HD>
-int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, bool vec, dim3 grid, int32_t *status, cudaStream_t st) {
+int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, int64_t pages, int n_sm, bool vec, int32_t *status, cudaStream_t st) {
+    // heads of one block: more of them read the table's rows less often, as long as there are four blocks
+    // for every SM all the same
+    int heads = 8;
+    auto blocks_y = [&] { return 2 * ((c.n_kv + heads - 1) / heads) + (r.q ? (r.n_q + heads - 1) / heads : 0); };
+    const int64_t filled = std::min<int64_t>(pages * c.n_seq, r.n_rows / c.page + c.n_seq);  // pages with rows, about
+    while (heads > 1 && filled * blocks_y() < 4 * n_sm) heads /= 2;
+    const dim3 grid((unsigned)pages, blocks_y(), c.n_seq);
     const int items = c.page * (HD / 16);
-    if (items <= kAppendThreads) kv_append_kernel<T, HD, 1><<<grid, kAppendThreads, 0, st>>>(c, r, vec, status);
-    else if (items <= 2 * kAppendThreads) kv_append_kernel<T, HD, 2><<<grid, kAppendThreads, 0, st>>>(c, r, vec, status);
-    else kv_append_kernel<T, HD, 4><<<grid, kAppendThreads, 0, st>>>(c, r, vec, status);
+    if (items <= 256) kv_append_kernel<T, HD, 1, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
+    else if (items <= 512) kv_append_kernel<T, HD, 2, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
+    else kv_append_kernel<T, HD, 2, 512><<<grid, 512, 0, st>>>(c, r, heads, vec, status);
     CK(cudaGetLastError());
     return DFB_OK;
 }
@@ -245,11 +252,10 @@ extern "C" int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_
     if (r->q) vec = vec && vec_ok(r->q, r->type, r->q_tok, r->q_head) && vec_ok(r->q_out, r->type, r->q_out_tok, r->q_out_head);
     // pages a sequence's rows can touch: consecutive positions n / page + 2 at most, given positions any of them
     const int64_t most = r->pos ? c->max_pages : std::min<int64_t>(c->max_pages, ((int64_t)r->max_rows + c->page - 2) / c->page + 1);
-    const dim3 grid((unsigned)most, 2 * c->n_kv + (r->q ? r->n_q : 0), c->n_seq);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto t) {
         using T = decltype(t);
-        return c->head_dim == 64 ? append_t<T, 64>(*c, *r, vec, grid, status, st) : append_t<T, 128>(*c, *r, vec, grid, status, st);
+        return c->head_dim == 64 ? append_t<T, 64>(*c, *r, most, n_sm, vec, status, st) : append_t<T, 128>(*c, *r, most, n_sm, vec, status, st);
     };
     return r->type == T_F32 ? go(float()) : r->type == T_F16 ? go(__half()) : go(__nv_bfloat16());
 }
