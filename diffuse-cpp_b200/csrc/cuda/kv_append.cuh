@@ -13,8 +13,10 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../../include/diffuse_b200.h"
+#include "simd.cuh"
 
 namespace dfb {
 
@@ -63,6 +65,23 @@ __device__ __forceinline__ void store8(T *p, bool vec, const float (&v)[8]) {
     }
 }
 
+// Two consecutive elements as f32, and back.
+template <typename T>
+__device__ __forceinline__ float2 pair_at(const uint4 *v, int e) {
+    if constexpr (sizeof(T) == 4) return reinterpret_cast<const float2 *>(v)[e];
+    else if constexpr (std::is_same_v<T, __half>) return __half22float2(reinterpret_cast<const __half2 *>(v)[e]);
+    else {
+        const uint32_t u = reinterpret_cast<const uint32_t *>(v)[e];
+        return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    }
+}
+template <typename T>
+__device__ __forceinline__ void set_pair(uint4 *v, int e, float2 x) {
+    if constexpr (sizeof(T) == 4) reinterpret_cast<float2 *>(v)[e] = x;
+    else if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2 *>(v)[e] = __float22half2_rn(x);
+    else reinterpret_cast<__nv_bfloat162 *>(v)[e] = __float22bfloat162_rn(x);
+}
+
 // x c + y s rounded to odd: the f32 next to the exact value towards zero, with its last bit set
 // when the value lies between two f32.  One more rounding (to E4M3, f16, bf16 or f32's own
 // nearest, which `near` receives) then gives what rounding the exact value gives: a value next
@@ -82,11 +101,14 @@ __device__ __forceinline__ float rot_odd(float x, float c, float y, float s, flo
     return __uint_as_float(u | 1u);
 }
 
-// x c + y s within 1.5 units in the last place of it (the rounding error of one product is added back).
-__device__ __forceinline__ float rot_near(float x, float c, float y, float s) {
-    const float p = __fmul_rn(y, s), e = __fmaf_rn(y, s, -p);
-    const float f = __fmaf_rn(x, c, p);
-    return e == 0.f ? f : __fadd_rn(f, e);  // (keeps the sign of a zero)
+// (a c - b s, a s + b c) of two pairs, each within 1.5 units in the last place: a product's rounding
+// error is taken back.  (A zero error is +0 here, so that taking it back keeps the sign of a zero.)
+__device__ __forceinline__ void rot_near(float2 &a, float2 &b, float2 c, float2 s) {
+    const float2 minus = make_float2(-1.f, -1.f), ns = mul2(s, minus);
+    const float2 p = mul2(b, ns), q = mul2(a, s);
+    const float2 x = fma2(fma2(b, s, p), minus, fma2(a, c, p));
+    b = fma2(fma2(a, ns, q), minus, fma2(b, c, q));
+    a = x;
 }
 // A value that rot_near gives lies within this of the exact one, relative to it (four times the bound).
 constexpr float kRotTol = 4.76837158203125e-07f;  // 2^-21
@@ -120,29 +142,65 @@ __device__ __forceinline__ int lower_bound(const int32_t *pos, int lo, int hi, i
     return lo;
 }
 
-// The codes of eight values.
-__device__ __forceinline__ uint2 encode8(const float *v, float inv) {
-    uint2 w;
-    w.x = e4m3_pair(v[0] * inv, v[1] * inv) | e4m3_pair(v[2] * inv, v[3] * inv) << 16;
-    w.y = e4m3_pair(v[4] * inv, v[5] * inv) | e4m3_pair(v[6] * inv, v[7] * inv) << 16;
-    return w;
+// Eight elements and the eight that lie half a head further, as they are in memory.
+template <typename T>
+struct RawItem {
+    static constexpr int NV = sizeof(T) / 2;  // 16-byte pieces of eight elements
+    uint4 v[2 * NV];
+    __device__ __forceinline__ void load(const T *p, int hd, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                v[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+                v[NV + i] = __ldcs(reinterpret_cast<const uint4 *>(p + hd / 2) + i);
+            }
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                reinterpret_cast<T *>(v)[e] = p[e];
+                reinterpret_cast<T *>(v)[8 + e] = p[hd / 2 + e];
+            }
+    }
+    __device__ __forceinline__ void store(T *p, int hd, bool vec) const {
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                reinterpret_cast<uint4 *>(p)[i] = v[i];
+                reinterpret_cast<uint4 *>(p + hd / 2)[i] = v[NV + i];
+            }
+        } else
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                p[e] = reinterpret_cast<const T *>(v)[e];
+                p[hd / 2 + e] = reinterpret_cast<const T *>(v)[8 + e];
+            }
+    }
+    __device__ __forceinline__ float2 pair(int e) const { return pair_at<T>(v, e); }
+    __device__ __forceinline__ void set(int e, float2 x) { set_pair<T>(v, e, x); }
+};
+
+// The codes of eight values times f.
+__device__ __forceinline__ uint2 encode8(const float2 *v, float f) {
+    const float2 g = make_float2(f, f);
+    const float2 a = mul2(v[0], g), b = mul2(v[1], g), c = mul2(v[2], g), d = mul2(v[3], g);
+    return make_uint2(e4m3_pair(a.x, a.y) | e4m3_pair(b.x, b.y) << 16, e4m3_pair(c.x, c.y) | e4m3_pair(d.x, d.y) << 16);
 }
 
 // One block: the rows that fall into one page of one sequence (the blockIdx.x-th touched page of
-// sequence blockIdx.z), for `heads` K heads, V heads or query heads in turn (blockIdx.y).  An item is
-// eight values and their rotation partners; a thread holds its items' cos and sin for all the heads
-// and its values between the maximum and the conversion, so rows are read once and the table's rows
-// once for a group of heads.
+// sequence blockIdx.z), for `heads` K heads, V heads or query heads in turn (blockIdx.y).  A thread has
+// one item, eight values and their rotation partners: it holds the item's cos and sin for all the heads,
+// its values between the maximum and the conversion, and the next head's rows as they come, so rows are
+// read once and the table's rows once for a group of heads.
 //
 // Bound: memory (rows in, codes out), if the rotation is cheap: rot_odd's sixteen instructions a value
 // took 520 us for 32768 rows of 32 + 32 + 32 heads.  rot_near's four decide every code but those whose
 // value lies within kRotTol of a border of two codes (one in 10^5), and the scale unless the maximum
 // lies that near to 448 * 2^e; those are worked out again with rot_odd.
-template <typename T, int HD, int ITEMS, int kAppendThreads>
-__global__ void __launch_bounds__(kAppendThreads, 512 / kAppendThreads) kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, int heads, bool vec,
+template <typename T, int HD, int kAppendThreads>
+__global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 1024 || sizeof(T) == 2 ? 1024 / kAppendThreads : 512 / kAppendThreads) kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, int heads, bool vec,
                                                                       int32_t *status) {
     constexpr int IPR = HD / 16;  // items per row
-    __shared__ float red[2][kAppendThreads / 32];
+    __shared__ uint32_t red[3];
     __shared__ uint32_t written[4];
     const int s = blockIdx.z, P = c.page, tid = threadIdx.x;
     const int groups = (c.n_kv + heads - 1) / heads;  // blocks of the K heads
@@ -201,21 +259,24 @@ __global__ void __launch_bounds__(kAppendThreads, 512 / kAppendThreads) kv_appen
     const bool rotate = r.rope && sec != 1;
 
     if (tid < 4) written[tid] = 0;
+    if (tid < 3) red[tid] = 0;
     __syncthreads();
-    int slot[ITEMS];
-    float4 cs[ITEMS][4];
-    const T *src[ITEMS];
-#pragma unroll
-    for (int j = 0; j < ITEMS; j++) {
-        const int it = tid + j * kAppendThreads, row = lo + it / IPR, i = (it % IPR) * 8;
-        slot[j] = row < hi ? slot_of(row) : -1;
-        src[j] = src0 + row * tok + i;
-        if (slot[j] < 0) continue;
-        if (i == 0) atomicOr(&written[slot[j] >> 5], 1u << (slot[j] & 31));
+    const int row = lo + tid / IPR, i = (tid % IPR) * 8, slot = row < hi ? slot_of(row) : -1;
+    const T *src = src0 + row * tok + i;
+    auto table = [&] { return r.rope + ((size_t)(p0 + slot) * (HD / 2) + i) * 2; };  // the item's cos and sin
+    float2 cs[4], sn[4];
+    RawItem<T> raw;
+    if (slot >= 0) {
+        raw.load(src + head0 * head_st, HD, vec);
+        if (i == 0) atomicOr(&written[slot >> 5], 1u << (slot & 31));
         if (rotate) {
-            const float4 *t = reinterpret_cast<const float4 *>(r.rope + ((size_t)(p0 + slot[j]) * (HD / 2) + i) * 2);
+            const float4 *t = reinterpret_cast<const float4 *>(table());
 #pragma unroll
-            for (int e = 0; e < 4; e++) cs[j][e] = __ldg(t + e);
+            for (int e = 0; e < 4; e++) {
+                const float4 v = __ldg(t + e);
+                cs[e] = make_float2(v.x, v.z);
+                sn[e] = make_float2(v.y, v.w);
+            }
         }
     }
     __syncthreads();
@@ -225,103 +286,83 @@ __global__ void __launch_bounds__(kAppendThreads, 512 / kAppendThreads) kv_appen
         const uint32_t all = kept - t >= 32 ? 0xffffffffu : (1u << (kept - t)) - 1;
         survive |= (all & ~written[t >> 5]) != 0;
     }
-    // item j of a head: its 16 values, rotated within kRotTol, or (exact) rounded to odd
-    auto item = [&](int j, int head, bool exact, float (&x)[16]) {
-        float u[8], w[8];
-        load8(src[j] + head * head_st, vec, u);
-        load8(src[j] + head * head_st + HD / 2, vec, w);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float cc = e & 1 ? cs[j][e / 2].z : cs[j][e / 2].x, ss = e & 1 ? cs[j][e / 2].w : cs[j][e / 2].y;
-            float n;
-            x[e] = !rotate ? u[e] : exact ? rot_odd(u[e], cc, w[e], -ss, n) : rot_near(u[e], cc, w[e], -ss);
-            x[8 + e] = !rotate ? w[e] : exact ? rot_odd(u[e], ss, w[e], cc, n) : rot_near(u[e], ss, w[e], cc);
-        }
+    // value e of the item or its partner, rounded to odd; near: to the nearest f32
+    auto exact = [&](int head, int e, bool second, float &near) {
+        const T *p = src + head * head_st + e;
+        const float u = to_f32<T>(p[0]), w = to_f32<T>(p[HD / 2]), cc = table()[2 * e], ss = table()[2 * e + 1];
+        return second ? rot_odd(u, ss, w, cc, near) : rot_odd(u, cc, w, -ss, near);
     };
-    // finite values only, and their maximum
-    auto clean = [&](float (&x)[16], float &amax, bool &bad) {
-        float m = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; e++) m = fmaxf(m, fabsf(x[e]));
-        bool all = m < INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; e++) all = all && x[e] == x[e];
-        if (!all) {
-            bad = true;
-            m = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                if (x[e] != x[e]) x[e] = 0.f;
-                if (fabsf(x[e]) < INFINITY) m = fmaxf(m, fabsf(x[e]));
-            }
-        }
-        amax = fmaxf(amax, m);
-    };
-    auto block_max = [&](float v, int buf) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-        if ((tid & 31) == 0) red[buf][tid >> 5] = v;
+    // The block's maximum of values >= 0, for head n of the block: their bits, which have the same order.
+    // Three words take turns, so that one barrier a head is enough: the one that head n - 1 has read is
+    // cleared for head n + 2.
+    auto block_max = [&](float v, int n) {
+        const uint32_t u = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+        if ((tid & 31) == 0) atomicMax(&red[n % 3], u);
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kAppendThreads / 32; w++) v = fmaxf(v, red[buf][w]);
-        return v;
+        if (tid == 0) red[(n + 2) % 3] = 0;
+        return __uint_as_float(red[n % 3]);
     };
-    if (sec == 2) {
-        for (int head = head0; head < head1; head++)
-#pragma unroll
-            for (int j = 0; j < ITEMS; j++) {
-                if (slot[j] < 0) continue;
-                const int it = tid + j * kAppendThreads, row = lo + it / IPR, i = (it % IPR) * 8;
-                float x[16];
-                if constexpr (sizeof(T) == 4) {  // f32 rows: the nearest f32 of the exact value
-                    float u[8], w[8];
-                    load8(src[j] + head * head_st, vec, u);
-                    load8(src[j] + head * head_st + HD / 2, vec, w);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float cc = e & 1 ? cs[j][e / 2].z : cs[j][e / 2].x, ss = e & 1 ? cs[j][e / 2].w : cs[j][e / 2].y;
-                        x[e] = u[e];
-                        x[8 + e] = w[e];
-                        if (rotate) {
-                            rot_odd(u[e], cc, w[e], -ss, x[e]);
-                            rot_odd(u[e], ss, w[e], cc, x[8 + e]);
-                        }
-                    }
-                } else {
-                    item(j, head, false, x);
-                }
-                T *dst = reinterpret_cast<T *>(r.q_out) + row * r.q_out_tok + head * r.q_out_head + i;
-                store8(dst, vec, reinterpret_cast<float(&)[8]>(x[0]));
-                store8(dst + HD / 2, vec, reinterpret_cast<float(&)[8]>(x[8]));
-            }
-        return;
-    }
     bool bad = false;
     for (int head = head0; head < head1; head++) {
+        float2 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = raw.pair(e);
+        if (slot >= 0 && head + 1 < head1) raw.load(src + (head + 1) * head_st, HD, vec);
+        if (rotate) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (sizeof(T) == 4 && sec == 2) {  // f32 rows for the caller: the nearest f32
+                    const float2 a = x[e], b = x[4 + e];
+                    rot_odd(a.x, cs[e].x, b.x, -sn[e].x, x[e].x);
+                    rot_odd(a.y, cs[e].y, b.y, -sn[e].y, x[e].y);
+                    rot_odd(a.x, sn[e].x, b.x, cs[e].x, x[4 + e].x);
+                    rot_odd(a.y, sn[e].y, b.y, cs[e].y, x[4 + e].y);
+                } else rot_near(x[e], x[4 + e], cs[e], sn[e]);
+            }
+        }
+        if (sec == 2) {
+            if (slot < 0) continue;
+            T *dst = reinterpret_cast<T *>(r.q_out) + row * r.q_out_tok + head * r.q_out_head + i;
+            RawItem<T> y;
+#pragma unroll
+            for (int e = 0; e < 8; e++) y.set(e, x[e]);
+            y.store(dst, HD, vec);
+            continue;
+        }
         const size_t blk = (size_t)pid * c.n_kv + head;
         float *scale = (sec == 0 ? c.k_scale : c.v_scale) + blk;
         uint8_t *codes = reinterpret_cast<uint8_t *>(sec == 0 ? c.k : c.v) + blk * P * HD;
         const int old = survive ? scale_exp(*scale) : 0;  // (every thread has it before block_max lets one write)
-        float x[ITEMS][16], amax = 0.f;
+        float amax = 0.f;
+        if (slot >= 0) {
 #pragma unroll
-        for (int j = 0; j < ITEMS; j++) {
-            if (slot[j] < 0) continue;
-            item(j, head, false, x[j]);
-            clean(x[j], amax, bad);
+            for (int e = 0; e < 8; e++) amax = max3_nan(amax, fabsf(x[e].x), fabsf(x[e].y));
+            if (!(amax < INFINITY)) {  // the finite values' maximum; NaN is stored as 0, infinities as the largest code
+                bad = true;
+                amax = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x[e].x = x[e].x != x[e].x ? 0.f : x[e].x;
+                    x[e].y = x[e].y != x[e].y ? 0.f : x[e].y;
+                    amax = fmaxf(amax, fmaxf(fabsf(x[e].x) < INFINITY ? fabsf(x[e].x) : 0.f, fabsf(x[e].y) < INFINITY ? fabsf(x[e].y) : 0.f));
+                }
+            }
         }
-        amax = block_max(amax, head & 1);
+        amax = block_max(amax, head - head0);
         if (rotate && need_exp(amax * (1.f - kRotTol)) != need_exp(amax * (1.f + kRotTol))) {  // (the same for the whole block)
             amax = 0.f;
-#pragma unroll
-            for (int j = 0; j < ITEMS; j++) {
-                if (slot[j] < 0) continue;
-                float y[16];
-                item(j, head, true, y);
-                clean(y, amax, bad);
+            if (slot >= 0) {
+#pragma unroll 1
+                for (int e = 0; e < 16; e++) {
+                    float n;
+                    const float v = fabsf(exact(head, e & 7, e & 8, n));
+                    if (v < INFINITY) amax = fmaxf(amax, v);
+                }
             }
             __syncthreads();
-            amax = block_max(amax, head & 1);
+            if (tid == 0) red[(head - head0) % 3] = 0;
             __syncthreads();
+            amax = block_max(amax, head - head0);
         }
         int e = need_exp(amax);
         if (survive) {
@@ -339,27 +380,26 @@ __global__ void __launch_bounds__(kAppendThreads, 512 / kAppendThreads) kv_appen
             }
         }
         if (tid == 0) *scale = exp2i(e);
+        if (slot < 0) continue;
         const float inv = exp2i(-e);
-#pragma unroll
-        for (int j = 0; j < ITEMS; j++) {
-            if (slot[j] < 0) continue;
-            uint8_t *dst = codes + slot[j] * HD + ((tid + j * kAppendThreads) % IPR) * 8;
-            uint2 w0 = encode8(&x[j][0], inv), w1 = encode8(&x[j][8], inv);
-            if (rotate) {
-                const float up = inv * (1.f + kRotTol), down = inv * (1.f - kRotTol);
-                const uint2 a0 = encode8(&x[j][0], up), a1 = encode8(&x[j][8], up), b0 = encode8(&x[j][0], down), b1 = encode8(&x[j][8], down);
-                if (a0.x != b0.x || a0.y != b0.y || a1.x != b1.x || a1.y != b1.y) {
-                    float y[16], m = 0.f;
-                    bool ignored = false;
-                    item(j, head, true, y);
-                    clean(y, m, ignored);
-                    w0 = encode8(&y[0], inv);
-                    w1 = encode8(&y[8], inv);
+        uint8_t *dst = codes + slot * HD + i;
+        // rotated: a little more and a little less have the same code, or a border lies between
+        const float up = rotate ? inv * (1.f + kRotTol) : inv, down = rotate ? inv * (1.f - kRotTol) : inv;
+        const uint2 w0 = encode8(&x[0], up), w1 = encode8(&x[4], up);
+        if (rotate) {
+            const uint2 b0 = encode8(&x[0], down), b1 = encode8(&x[4], down);
+            if ((w0.x ^ b0.x) | (w0.y ^ b0.y) | (w1.x ^ b1.x) | (w1.y ^ b1.y)) {
+#pragma unroll 1
+                for (int e = 0; e < 16; e++) {
+                    float n;
+                    const float v = exact(head, e & 7, e & 8, n);
+                    dst[(e & 8) * (HD / 16) + (e & 7)] = (uint8_t)e4m3_pair(v != v ? 0.f : v * inv, 0.f);
                 }
+                continue;
             }
-            *reinterpret_cast<uint2 *>(dst) = w0;
-            *reinterpret_cast<uint2 *>(dst + HD / 2) = w1;
         }
+        *reinterpret_cast<uint2 *>(dst) = w0;
+        *reinterpret_cast<uint2 *>(dst + HD / 2) = w1;
     }
     if (bad) flag(DFB_STAT_NONFINITE);
 }

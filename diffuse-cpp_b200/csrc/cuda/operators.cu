@@ -105,9 +105,9 @@ int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, int64_t pages, int n_s
     while (heads > 1 && filled * blocks_y() < 4 * n_sm) heads /= 2;
     const dim3 grid((unsigned)pages, blocks_y(), c.n_seq);
     const int items = c.page * (HD / 16);
-    if (items <= 256) kv_append_kernel<T, HD, 1, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
-    else if (items <= 512) kv_append_kernel<T, HD, 2, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
-    else kv_append_kernel<T, HD, 2, 512><<<grid, 512, 0, st>>>(c, r, heads, vec, status);
+    if (items <= 256) kv_append_kernel<T, HD, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
+    else if (items <= 512) kv_append_kernel<T, HD, 512><<<grid, 512, 0, st>>>(c, r, heads, vec, status);
+    else kv_append_kernel<T, HD, 1024><<<grid, 1024, 0, st>>>(c, r, heads, vec, status);
     CK(cudaGetLastError());
     return DFB_OK;
 }
