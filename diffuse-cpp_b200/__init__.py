@@ -118,6 +118,7 @@ def _load():
         (dfc, "dfc_context_free"): (None, [P]),
         (dfc, "dfc_context_engine"): (P, [P]),
         (dfc, "dfc_forward"): (I, [P, P, I, P]),
+        (dfc, "dfc_score"): (I, [P, P, I, P, I, P, P, P, P]),
         (dfc, "dfc_generate"): (I, [P, P, I, I, C.POINTER(SamplerParams), P, C.POINTER(Trace)]),
         (dfc, "dfc_quantize_file"): (I, [C.c_char_p, C.c_char_p, C.c_char_p, I]),
         (dfc, "dfc_synth_model"): (I, [C.c_char_p, C.POINTER(SynthSpec)]),
@@ -277,6 +278,30 @@ class Context:
         if not native()[1].dfc_forward(self._h, _ptr(t), t.size, _ptr(out)):
             raise DiffuseError(_dfc_err())
         return out
+
+    def score(self, tokens, targets=None, top_k: int = 0) -> dict:
+        """Log probabilities of targets [n] at the positions of tokens [n] (negative: 0; None: not
+        asked for), the distributions' entropies in nats, and the top_k <= 32 most probable tokens:
+        {"logprob": [n] or None, "entropy": [n], "top_ids": [n, top_k], "top_logprob": [n, top_k]}.
+        One forward; its logits stay on the GPU.  A masked position's score is that of what the
+        model would write there; a shifted model (Dream) predicts position i from row i - 1."""
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        if t.ndim != 1 or not t.size:
+            raise ValueError("tokens must be a non-empty list")
+        lp = tg = None
+        if targets is not None:
+            tg = np.ascontiguousarray(targets, dtype=np.int32)
+            if tg.shape != t.shape:
+                raise ValueError(f"{tg.shape} targets for {t.shape} tokens")
+            lp = np.empty(t.size, np.float32)
+        if not 0 <= top_k <= 32:
+            raise ValueError("top_k must be 0..32")
+        ent = np.empty(t.size, np.float32)
+        ids, tlp = np.empty((t.size, top_k), np.int32), np.empty((t.size, top_k), np.float32)
+        if native()[1].dfc_score(self._h, _ptr(t), t.size, None if tg is None else _ptr(tg), top_k,
+                                 None if lp is None else _ptr(lp), _ptr(ent), _ptr(ids), _ptr(tlp)) != 0:
+            raise DiffuseError(_dfc_err())
+        return {"logprob": lp, "entropy": ent, "top_ids": ids, "top_logprob": tlp}
 
     def linear(self, role: int, layer: int, x: np.ndarray) -> np.ndarray:
         """y = x . W^T through the production dequant GEMM (for parity tests)."""

@@ -720,6 +720,8 @@ extern "C" int dfb_model_bytes(const dfb_model *m, size_t *bytes) {
 }
 
 // ───────────────────────── context ─────────────────────────
+constexpr int kScoreTop = 32;  // most alternatives of dfb_token_logprobs
+
 struct dfb_ctx {
     dfb_model *m = nullptr;
     cudaStream_t st = nullptr;
@@ -765,6 +767,10 @@ struct dfb_ctx {
     std::vector<ProfRec> prof_pending;
     std::vector<cudaEvent_t> ev_pool;
     dfb_prof_entry prof_acc[DFB_PROF_N]{};
+    // dfb_score: the alternatives of each position
+    int32_t *score_ids = nullptr;
+    float *score_lp = nullptr;
+    int score_cap = 0;
     // generation
     bool gen_active = false;
     int total = 0;                   // positions of all segments
@@ -779,8 +785,11 @@ static void ctx_free_buffers(dfb_ctx *c) {
                   c->last_changed, c->cand_tok, c->commit_pos, c->commit_tok, c->order, c->masked, c->active_pos,
                   c->masked_pos, c->cnt, c->cand_conf, c->cand_ent, c->ws, c->tile_cnt, c->err, c->seg_off,
                   c->seg_cnt, c->sched, c->tmp_active, c->tmp_masked, c->rope_pos, c->masked_row, c->done, c->tiles,
-                  c->unif, c->tp_stats, c->tp_gath, c->tp_g};
+                  c->unif, c->tp_stats, c->tp_gath, c->tp_g, c->score_ids, c->score_lp};
     for (void *p : ps) cudaFree(p);
+    c->score_ids = nullptr;
+    c->score_lp = nullptr;
+    c->score_cap = 0;
     c->seg_off = c->seg_cnt = c->sched = c->tmp_active = c->tmp_masked = c->rope_pos = c->masked_row = nullptr;
     c->done = nullptr;
     c->tiles = nullptr;
@@ -1209,9 +1218,8 @@ static int prepare_step(dfb_ctx *c, int full, int step, int keep_active) {
     return DFB_OK;
 }
 
-extern "C" int dfb_forward(dfb_ctx *c, const int32_t *tokens, int n, float *logits_host) {
-    if (!c || !tokens || !logits_host || n <= 0) return set_err(DFB_ERR_ARG, "bad arguments");
-    std::lock_guard<std::mutex> lk(device_lock(c->m->device));
+// Full forward over n host tokens, launched on the context's stream; c->logits gets their rows.
+static int forward_tokens(dfb_ctx *c, const int32_t *tokens, int n) {
     CK(cudaSetDevice(c->m->device));
     const int V = c->m->hp.n_vocab;
     for (int i = 0; i < n; i++)
@@ -1222,15 +1230,76 @@ extern "C" int dfb_forward(dfb_ctx *c, const int32_t *tokens, int n, float *logi
     CK(cudaMemcpyAsync(c->seq, tokens, n * sizeof(int32_t), cudaMemcpyHostToDevice, c->st));
     CK(cudaMemsetAsync(c->masked, 0, n, c->st));
     RET(prepare_step(c, 1, 0, 0));
-    RET(run_forward(c, n));
-    // (tensor parallelism: this rank's vocabulary columns, n x n_vocab_local)
-    CK(cudaMemcpyAsync(logits_host, c->logits, (size_t)n * c->m->n_vocab_l * sizeof(float), cudaMemcpyDeviceToHost, c->st));
+    return run_forward(c, n);
+}
+// Wait for a forward over n tokens and what follows it on the stream, and look at their errors.
+static int forward_finish(dfb_ctx *c, int n) {
     int verr = 0;
     CK(cudaMemcpyAsync(&verr, c->cnt + CNT_ERR, sizeof(int), cudaMemcpyDeviceToHost, c->st));
     CK(cudaStreamSynchronize(c->st));
     RET(check_values(c, verr));
     prof_collect(c, n);
     return check_err(c);
+}
+
+extern "C" int dfb_forward(dfb_ctx *c, const int32_t *tokens, int n, float *logits_host) {
+    if (!c || !tokens || !logits_host || n <= 0) return set_err(DFB_ERR_ARG, "bad arguments");
+    std::lock_guard<std::mutex> lk(device_lock(c->m->device));
+    RET(forward_tokens(c, tokens, n));
+    // (tensor parallelism: this rank's vocabulary columns, n x n_vocab_local)
+    CK(cudaMemcpyAsync(logits_host, c->logits, (size_t)n * c->m->n_vocab_l * sizeof(float), cudaMemcpyDeviceToHost, c->st));
+    return forward_finish(c, n);
+}
+
+extern "C" int dfb_score(dfb_ctx *c, const int32_t *tokens, int n, const int32_t *targets, int top_k, float *logprob,
+                         float *entropy, int32_t *top_ids, float *top_logprob) {
+    if (!c || !tokens || n <= 0 || !targets != !logprob) return set_err(DFB_ERR_ARG, "bad arguments");
+    const dfb_model *m = c->m;
+    if (m->tp_size > 1) return set_err(DFB_ERR_STATE, "dfb_score needs every vocabulary column on one GPU");
+    if (top_k < 0 || top_k > kScoreTop || top_k > m->hp.n_vocab || (top_k && (!top_ids || !top_logprob)))
+        return set_err(DFB_ERR_ARG, "top_k %d outside [0, %d], or without outputs", top_k, std::min(kScoreTop, m->hp.n_vocab));
+    for (int i = 0; targets && i < n; i++)
+        if (targets[i] >= m->hp.n_vocab) return set_err(DFB_ERR_ARG, "target %d at %d outside the vocabulary", targets[i], i);
+    std::vector<int32_t> rows(n);  // the logits row that predicts position i: a shifted model's is the one before
+    for (int i = 0; i < n; i++) rows[i] = m->hp.shift_logits && i > 0 ? i - 1 : i;
+    std::lock_guard<std::mutex> lk(device_lock(m->device));
+    RET(forward_tokens(c, tokens, n));
+    if (top_k && c->score_cap < c->cap) {
+        cudaFree(c->score_ids);
+        cudaFree(c->score_lp);
+        c->score_ids = nullptr;
+        c->score_lp = nullptr;
+        c->score_cap = 0;
+        CK(cudaMalloc(&c->score_ids, (size_t)c->cap * kScoreTop * sizeof(int32_t)));
+        CK(cudaMalloc(&c->score_lp, (size_t)c->cap * kScoreTop * sizeof(float)));
+        c->score_cap = c->cap;
+    }
+    dfb_logprob_args a{};
+    a.logits = c->logits;
+    a.type = G_F32;
+    a.n_vocab = m->hp.n_vocab;
+    a.n_rows = a.n_logits = n;
+    a.ld = m->n_vocab_l;
+    a.rows = c->order;  // (free between generation steps, like the candidates' values below)
+    CK(cudaMemcpyAsync(c->order, rows.data(), n * sizeof(int32_t), cudaMemcpyHostToDevice, c->st));
+    if (targets) {
+        a.targets = c->commit_tok;
+        a.logprob = c->cand_conf;
+        CK(cudaMemcpyAsync(c->commit_tok, targets, n * sizeof(int32_t), cudaMemcpyHostToDevice, c->st));
+    }
+    a.entropy = entropy ? c->cand_ent : nullptr;
+    a.top_k = top_k;
+    a.top_ids = c->score_ids;
+    a.top_logprob = c->score_lp;
+    RET(dfb_token_logprobs(&a, nullptr, c->st));
+    auto fetch = [&](void *dst, const void *src, size_t count) {
+        return dst && count ? cudaMemcpyAsync(dst, src, count * 4, cudaMemcpyDeviceToHost, c->st) : cudaSuccess;
+    };
+    CK(fetch(logprob, a.logprob, n));
+    CK(fetch(entropy, a.entropy, n));
+    CK(fetch(top_ids, a.top_ids, (size_t)n * top_k));
+    CK(fetch(top_logprob, a.top_logprob, (size_t)n * top_k));
+    return forward_finish(c, n);
 }
 
 extern "C" int dfb_linear(dfb_ctx *c, int role, int layer, const float *x_host, int M, float *y_host) {

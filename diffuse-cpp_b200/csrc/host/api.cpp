@@ -456,6 +456,13 @@ int dfc_forward(void *ctx, const int32_t *tokens, int n_tokens, float *logits_ou
     return 1;
 }
 
+int dfc_score(void *ctx, const int32_t *tokens, int n_tokens, const int32_t *targets, int top_k, float *logprob,
+              float *entropy, int32_t *top_ids, float *top_logprob) {
+    if (!ctx) return set_error(DFB_ERR_ARG, "null context");
+    const int r = dfb_score(((diffuse_context *)ctx)->dc, tokens, n_tokens, targets, top_k, logprob, entropy, top_ids, top_logprob);
+    return r == DFB_OK ? r : set_error(r, "%s", dfb_last_error());
+}
+
 int dfc_generate(void *ctx, const int32_t *prompt, int n_prompt, int n_generate, const dfb_sampler_params *p,
                  int32_t *out, dfc_trace *trace) {
     if (!ctx || !p || !out || n_generate <= 0 || n_prompt < 0) return set_error(DFB_ERR_ARG, "bad arguments");

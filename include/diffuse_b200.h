@@ -101,6 +101,15 @@ void dfb_ctx_free(dfb_ctx *c);
  * copied to the host buffer [n * n_vocab]. */
 int dfb_forward(dfb_ctx *c, const int32_t *tokens, int n, float *logits_host);
 
+/* Score a text: the forward of dfb_forward, then dfb_token_logprobs (below) on the logits where
+ * they lie, so a position costs a few numbers of copying instead of n_vocab.  For each position i:
+ * the log probability of targets[i] (negative: 0), the entropy (nats) and the top_k <= 32 most
+ * probable tokens with their log probabilities, all under the logits row that predicts position i
+ * (a shifted model's row i - 1 for i > 0, as the sampler reads it).  Host arrays [n], [n * top_k];
+ * targets and logprob, and entropy, may be NULL.  Not supported with tensor parallelism. */
+int dfb_score(dfb_ctx *c, const int32_t *tokens, int n, const int32_t *targets, int top_k, float *logprob, float *entropy,
+              int32_t *top_ids, float *top_logprob);
+
 /* One linear layer through the production dequant-fused GEMM: y[M x ne1] = x[M x ne0] . W^T
  * for a model weight (host buffers).  Exposed for parity tests of the GEMM alone. */
 int dfb_linear(dfb_ctx *c, int role, int layer, const float *x_host, int M, float *y_host);

@@ -42,6 +42,9 @@ void  dfc_context_free(void *ctx);
 void *dfc_context_engine(void *ctx);
 /* 1 on success, 0 on failure (like diffuse_forward's bool). */
 int   dfc_forward(void *ctx, const int32_t *tokens, int n_tokens, float *logits_out);
+/* dfb_score (diffuse_b200.h): log probabilities, entropies and alternatives; DFB_OK or an error code. */
+int   dfc_score(void *ctx, const int32_t *tokens, int n_tokens, const int32_t *targets, int top_k, float *logprob,
+                float *entropy, int32_t *top_ids, float *top_logprob);
 
 /* Per-step record filled by dfc_generate (arrays caller-allocated, may be NULL). */
 typedef struct {
