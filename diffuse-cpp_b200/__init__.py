@@ -106,6 +106,7 @@ def _load():
         (dfb, "dfb_gen_step_batch"): (I, [P, I, P, I, P, P]),
         (dfb, "dfb_gen_commits_batch"): (I, [P, P, P, P, I]),
         (dfc, "dfc_generate_batch"): (I, [P, P, P, I, I, C.POINTER(SamplerParams), P, P]),
+        (dfb, "dfb_ctx_set_kv8"): (I, [P, I]),
         (dfb, "dfb_ctx_stream"): (I, [P, C.POINTER(P)]),
         (dfc, "dfc_last_error"): (C.c_char_p, []),
         (dfc, "dfc_model_load"): (P, [C.c_char_p, I]),
@@ -263,12 +264,19 @@ class Model:
 class Context:
     """diffuse_context: device buffers + stream of one generation at a time."""
 
-    def __init__(self, model: Model, n_ctx: int = 0, n_threads: int = 4):
+    def __init__(self, model: Model, n_ctx: int = 0, n_threads: int = 4, kv_bits: int = 32):
+        """kv_bits 8: the K/V kept between steps in 8 bits (dfb_ctx_set_kv8; heads of 64 or 128)."""
+        if kv_bits not in (8, 32):
+            raise ValueError("kv_bits must be 8 or 32")
         self.model = model
         self._h = native()[1].dfc_context_new(model._h, n_ctx, n_threads)
         if not self._h:
             raise DiffuseError(_dfc_err())
         self.engine = native()[1].dfc_context_engine(self._h)
+        if kv_bits == 8 and native()[0].dfb_ctx_set_kv8(self.engine, 1) != 0:
+            msg = _dfb_err()
+            self.close()
+            raise DiffuseError(msg)
 
     def forward(self, tokens) -> np.ndarray:
         """diffuse_forward: logits [n, n_vocab] for n tokens (no cache); a tensor-parallel

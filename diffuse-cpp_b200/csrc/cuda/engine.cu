@@ -720,6 +720,7 @@ extern "C" int dfb_model_bytes(const dfb_model *m, size_t *bytes) {
 }
 
 // ───────────────────────── context ─────────────────────────
+constexpr int kKv8Page = 64;   // positions of one page of a context's 8-bit cache
 constexpr int kScoreTop = 32;  // most alternatives of dfb_token_logprobs
 
 struct dfb_ctx {
@@ -767,6 +768,18 @@ struct dfb_ctx {
     std::vector<ProfRec> prof_pending;
     std::vector<cudaEvent_t> ev_pool;
     dfb_prof_entry prof_acc[DFB_PROF_N]{};
+    // 8-bit cache (dfb_ctx_set_kv8): kc, vc then hold one layer's fresh rows, in row order
+    struct Kv8 {
+        bool on = false;
+        uint8_t *codes = nullptr;  // [2][layer][page][KV head][64][head_dim]
+        float *scale = nullptr;    // [2][layer][page][KV head]
+        int32_t *pages = nullptr, *row_off = nullptr, *len = nullptr, *status = nullptr;
+        int *iota = nullptr;
+        __half *q = nullptr, *o = nullptr;
+        uint8_t *ws = nullptr;
+        size_t page_cap = 0, table_cap = 0, ws_bytes = 0;
+        int n_pages = 0, max_pages = 0, max_len = 0;
+    } kv8;
     // dfb_score: the alternatives of each position
     int32_t *score_ids = nullptr;
     float *score_lp = nullptr;
@@ -785,8 +798,13 @@ static void ctx_free_buffers(dfb_ctx *c) {
                   c->last_changed, c->cand_tok, c->commit_pos, c->commit_tok, c->order, c->masked, c->active_pos,
                   c->masked_pos, c->cnt, c->cand_conf, c->cand_ent, c->ws, c->tile_cnt, c->err, c->seg_off,
                   c->seg_cnt, c->sched, c->tmp_active, c->tmp_masked, c->rope_pos, c->masked_row, c->done, c->tiles,
-                  c->unif, c->tp_stats, c->tp_gath, c->tp_g, c->score_ids, c->score_lp};
+                  c->unif, c->tp_stats, c->tp_gath, c->tp_g, c->score_ids, c->score_lp, c->kv8.codes,
+                  c->kv8.scale, c->kv8.pages, c->kv8.row_off, c->kv8.len, c->kv8.status, c->kv8.iota, c->kv8.q, c->kv8.o,
+                  c->kv8.ws};
     for (void *p : ps) cudaFree(p);
+    const bool kv8_on = c->kv8.on;
+    c->kv8 = dfb_ctx::Kv8{};
+    c->kv8.on = kv8_on;
     c->score_ids = nullptr;
     c->score_lp = nullptr;
     c->score_cap = 0;
@@ -825,7 +843,7 @@ static int ctx_reserve(dfb_ctx *c, int n) {
     const int cap = std::max(n, 64);
     ctx_free_buffers(c);
     // per-rank widths: FFN features and vocabulary rows of this rank (all of them at tp_size 1)
-    const size_t d = hp.n_embd, ff = m->n_ff_l, V = m->n_vocab_l, L = hp.n_layer, kvd = m->n_kv, hd = m->hd;
+    const size_t d = hp.n_embd, ff = m->n_ff_l, V = m->n_vocab_l, L = c->kv8.on ? 1 : hp.n_layer, kvd = m->n_kv, hd = m->hd;
 #define AL(ptr, count) CK(cudaMalloc(&(ptr), sizeof(*(ptr)) * (size_t)(count)))
     AL(c->x, cap * d); AL(c->y, cap * d); AL(c->h, 4 * cap * d); AL(c->att, 4 * cap * d); AL(c->q, cap * d);
     AL(c->ffh, 4 * cap * ff);
@@ -838,6 +856,14 @@ static int ctx_reserve(dfb_ctx *c, int n) {
     AL(c->tmp_active, cap); AL(c->tmp_masked, cap); AL(c->rope_pos, cap); AL(c->masked_row, cap);
     AL(c->tiles, cap / kAttnRows + kMaxSeg + 1);
     AL(c->ws, (size_t)m->n_sm * 2 * kWsTile); AL(c->err, 1);
+    if (c->kv8.on) {
+        AL(c->kv8.row_off, kMaxSeg + 1); AL(c->kv8.len, kMaxSeg); AL(c->kv8.status, 1); AL(c->kv8.iota, cap);
+        AL(c->kv8.q, (size_t)cap * m->n_q); AL(c->kv8.o, (size_t)cap * m->n_q);
+        std::vector<int> iota(cap);
+        for (int i = 0; i < cap; i++) iota[i] = i;
+        CK(cudaMemcpy(c->kv8.iota, iota.data(), sizeof(int) * cap, cudaMemcpyHostToDevice));
+        CK(cudaMemset(c->kv8.status, 0, sizeof(int32_t)));
+    }
     const int n_mg_max = (cap + kMaxTok - 1) / kMaxTok;
     int max_tiles = m->lm_head.n_tiles;
     for (auto &Lw : m->layers) max_tiles = std::max({max_tiles, Lw.qkv.n_tiles, Lw.gateup.n_tiles, Lw.o.n_tiles, Lw.down.n_tiles});
@@ -1023,6 +1049,120 @@ static int launch_attn_t(dfb_ctx *c, const float *kc, const float *vc, int n_key
     return DFB_OK;
 }
 
+// 8-bit cache: layer l's pages, and the arguments of its two calls.
+static dfb_kv_cache kv8_cache(const dfb_ctx *c, int l) {
+    const dfb_model *m = c->m;
+    const size_t L = m->hp.n_layer, scales = (size_t)c->kv8.n_pages * (m->n_kv / m->hd), codes = scales * kKv8Page * m->hd;
+    dfb_kv_cache k{};
+    k.k = c->kv8.codes + l * codes;
+    k.v = c->kv8.codes + (L + l) * codes;
+    k.k_scale = c->kv8.scale + l * scales;
+    k.v_scale = c->kv8.scale + (L + l) * scales;
+    k.pages = c->kv8.pages;
+    k.n_pages = c->kv8.n_pages;
+    k.n_kv = m->n_kv / m->hd;
+    k.head_dim = m->hd;
+    k.page = kKv8Page;
+    k.n_seq = c->n_seg;
+    k.max_pages = c->kv8.max_pages;
+    return k;
+}
+static dfb_kv_attn kv8_attn(const dfb_ctx *c) {
+    const dfb_model *m = c->m;
+    dfb_kv_attn a{};
+    a.q = c->kv8.q;
+    a.out = c->kv8.o;
+    a.type = G_F16;
+    a.n_q = m->n_q / m->hd;
+    a.n_rows = c->total;
+    a.max_rows = a.max_keys = c->kv8.max_len;
+    a.scale = 1.0f / sqrtf((float)m->hd);
+    a.q_tok = a.out_tok = m->n_q;
+    a.q_head = a.out_head = m->hd;
+    a.row_off = c->kv8.row_off;
+    a.len = c->kv8.len;
+    return a;
+}
+// Pages for the segments, one after another, and the attention's workspace.
+static int kv8_layout(dfb_ctx *c) {
+    const dfb_model *m = c->m;
+    auto &k = c->kv8;
+    const size_t L = m->hp.n_layer;
+    std::vector<int32_t> len(c->n_seg);
+    k.n_pages = k.max_pages = k.max_len = 0;
+    for (int s = 0; s < c->n_seg; s++) {
+        len[s] = c->seg_off_h[s + 1] - c->seg_off_h[s];
+        const int n = (len[s] + kKv8Page - 1) / kKv8Page;
+        k.n_pages += n;
+        k.max_pages = std::max(k.max_pages, n);
+        k.max_len = std::max(k.max_len, len[s]);
+    }
+    const size_t table = (size_t)c->n_seg * k.max_pages;
+    if ((size_t)k.n_pages > k.page_cap) {
+        cudaFree(k.codes);
+        cudaFree(k.scale);
+        k.codes = nullptr;
+        k.scale = nullptr;
+        k.page_cap = 0;
+        CK(cudaMalloc(&k.codes, 2 * L * k.n_pages * kKv8Page * m->n_kv));
+        CK(cudaMalloc(&k.scale, 2 * L * k.n_pages * (m->n_kv / m->hd) * sizeof(float)));
+        k.page_cap = k.n_pages;
+    }
+    if (table > k.table_cap) {
+        cudaFree(k.pages);
+        k.pages = nullptr;
+        k.table_cap = 0;
+        CK(cudaMalloc(&k.pages, table * sizeof(int32_t)));
+        k.table_cap = table;
+    }
+    std::vector<int32_t> pages(table, 0);
+    for (int s = 0, at = 0; s < c->n_seg; s++)
+        for (int i = 0; i * kKv8Page < len[s]; i++) pages[(size_t)s * k.max_pages + i] = at++;
+    CK(cudaMemcpyAsync(k.pages, pages.data(), table * sizeof(int32_t), cudaMemcpyHostToDevice, c->st));
+    CK(cudaMemcpyAsync(k.len, len.data(), len.size() * sizeof(int32_t), cudaMemcpyHostToDevice, c->st));
+    size_t need = 0;
+    const dfb_kv_cache kc = kv8_cache(c, 0);
+    const dfb_kv_attn a = kv8_attn(c);
+    RET(dfb_kv_attention_workspace(&kc, &a, &need));
+    if (need > k.ws_bytes) {
+        cudaFree(k.ws);
+        k.ws = nullptr;
+        k.ws_bytes = 0;
+        CK(cudaMalloc(&k.ws, need));
+        k.ws_bytes = need;
+    }
+    return DFB_OK;
+}
+// Store layer l's fresh K and V rows and attend over its cache.  Every forward of a fresh sequence
+// writes all its positions, so a page's scale starts from the values it holds.
+static int kv8_step(dfb_ctx *c, int l) {
+    const dfb_model *m = c->m;
+    const dfb_kv_cache kc = kv8_cache(c, l);
+    const dfb_kv_attn a = kv8_attn(c);
+    dfb_kv_rows r{};
+    r.k = c->kc;
+    r.v = c->vc;
+    r.type = G_F32;
+    r.n_rows = c->total;
+    r.max_rows = c->kv8.max_len;
+    r.k_tok = r.v_tok = m->n_kv;
+    r.k_head = r.v_head = m->hd;
+    r.row_off = c->kv8.row_off;
+    r.len = c->kv8.len;
+    r.pos = c->rope_pos;
+    cudaEvent_t ev0 = nullptr;
+    prof_begin(c, &ev0);
+    RET(dfb_kv_append(&kc, &r, c->kv8.status, c->st));
+    rows_half_kernel<<<c->total, 256, 0, c->st>>>(c->q, m->n_q, c->cnt, c->kv8.q);
+    CK(cudaGetLastError());
+    RET(dfb_kv_attention(&kc, &a, c->kv8.ws, c->kv8.ws_bytes, c->kv8.status, c->st));
+    rows_pair_kernel<<<c->total, 256, 0, c->st>>>(c->kv8.o, m->n_q, c->cnt, c->att);
+    CK(cudaGetLastError());
+    // algorithmic bytes: K and V of every key once (8 bits), Q and the fresh rows in (f32), O out (pair rows)
+    prof_end(c, ev0, DFB_PROF_ATTN, 4.0 * c->total * m->n_q, 2.0 * c->total * m->n_kv, 8.0 * m->n_q + 8.0 * m->n_kv);
+    return DFB_OK;
+}
+
 // Tensor parallelism: the O and down projections are row-parallel (each rank holds the input
 // columns of its heads / FFN features), so y holds partial sums; an NCCL all-reduce over the
 // context's rows makes it the whole projection on every rank before the RMSNorm that adds it
@@ -1058,7 +1198,8 @@ static int run_forward(dfb_ctx *c, int n_total) {
     CK(cudaGetLastError());
     for (int l = 0; l < hp.n_layer; l++) {
         const LayerW &L = m->layers[l];
-        float *kc = c->kc + (size_t)l * cap * m->n_kv, *vc = c->vc + (size_t)l * cap * m->n_kv;
+        const size_t layer = c->kv8.on ? 0 : (size_t)l * cap * m->n_kv;
+        float *kc = c->kc + layer, *vc = c->vc + layer;
         // the previous layer's down projection is added to the residual stream here
         CK(launch_k(rmsnorm_kernel, dim3(cap), dim3(256), 0, c->st, true, c->x, (const float *)(l ? c->y : nullptr),
                     (const float *)L.attn_norm, d, hp.rms_norm_eps, (const int *)c->cnt, c->h));
@@ -1067,9 +1208,11 @@ static int run_forward(dfb_ctx *c, int n_total) {
         e.k_cache = kc; e.v_cache = vc; e.ld_kv = m->n_kv;
         e.n_q_tiles = m->nq_pad / 128; e.n_k_tiles = m->nk_pad / 128;
         e.n_q = m->n_q; e.n_kv = m->n_kv; e.head_dim = m->hd;
-        e.bias = L.bias_qkv; e.rope = c->rope; e.pos = c->active_pos; e.rope_pos = c->rope_pos;
+        e.bias = L.bias_qkv; e.rope = c->rope; e.rope_pos = c->rope_pos;
+        e.pos = c->kv8.on ? c->kv8.iota : c->active_pos;
         RET(launch_gemm<EPI_QKV>(c, L.qkv, c->xm_h, e));
-        switch (m->hd) {
+        if (c->kv8.on) RET(kv8_step(c, l));
+        else switch (m->hd) {
             case 16: RET(launch_attn_t<16>(c, kc, vc, n_total)); break;
             case 32: RET(launch_attn_t<32>(c, kc, vc, n_total)); break;
             case 64: RET(launch_attn_t<64>(c, kc, vc, n_total)); break;
@@ -1132,6 +1275,14 @@ static std::mutex &device_lock(int device) { return g_device_mu[device & 63]; }
 
 static int check_err(dfb_ctx *c) {
     int e = 0;
+    if (c->kv8.on) {
+        CK(cudaMemcpy(&e, c->kv8.status, sizeof(int), cudaMemcpyDeviceToHost));
+        if (e) {
+            cudaMemset(c->kv8.status, 0, sizeof(int));
+            if (e & DFB_STAT_TIMEOUT) return set_err(DFB_ERR_TIMEOUT, "attention over the 8-bit cache stopped; results of this call are invalid");
+            return set_err(DFB_ERR_ARG, "8-bit cache: %s (status %d)", e & DFB_STAT_NONFINITE ? "K or V not finite" : "bad rows", e);
+        }
+    }
     CK(cudaMemcpy(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost));
     if (e) {
         cudaMemset(c->err, 0, sizeof(int));
@@ -1174,6 +1325,20 @@ extern "C" void dfb_ctx_free(dfb_ctx *c) {
     delete c;
 }
 
+extern "C" int dfb_ctx_set_kv8(dfb_ctx *c, int on) {
+    if (!c) return set_err(DFB_ERR_ARG, "null context");
+    if (on && c->m->hd != 64 && c->m->hd != 128)
+        return set_err(DFB_ERR_UNSUPPORTED, "the 8-bit cache holds heads of 64 or 128, the model's have %d", c->m->hd);
+    std::lock_guard<std::mutex> lk(device_lock(c->m->device));
+    CK(cudaSetDevice(c->m->device));
+    CK(cudaStreamSynchronize(c->st));
+    const int cap = c->cap;
+    ctx_free_buffers(c);
+    c->gen_active = false;
+    c->kv8.on = on != 0;
+    return cap ? ctx_reserve(c, cap) : DFB_OK;
+}
+
 extern "C" int dfb_ctx_profile(dfb_ctx *c, int enable) {
     if (!c) return set_err(DFB_ERR_ARG, "null context");
     CK(cudaStreamSynchronize(c->st));
@@ -1203,7 +1368,7 @@ static int set_segments(dfb_ctx *c, const std::vector<int> &off) {
     c->n_seg = n;
     c->seg_off_h = off;
     c->total = off.back();
-    return DFB_OK;
+    return c->kv8.on ? kv8_layout(c) : DFB_OK;
 }
 
 // Active sets and work lists of one step over all segments (seg_prepare + seg_compact).
@@ -1215,6 +1380,10 @@ static int prepare_step(dfb_ctx *c, int full, int step, int keep_active) {
     CK(launch_k(seg_compact_kernel, dim3(1), dim3(1024), 0, c->st, false, c->n_seg, (const int *)c->seg_off,
                 (const int *)c->tmp_active, (const int *)c->tmp_masked, c->seg_cnt, c->m->hp.shift_logits, c->active_pos,
                 c->rope_pos, c->masked_pos, c->masked_row, c->tiles, c->cnt));
+    if (c->kv8.on) {
+        seg_row_off_kernel<<<1, 256, 0, c->st>>>(c->n_seg, c->seg_cnt, c->cnt, c->kv8.row_off);
+        CK(cudaGetLastError());
+    }
     return DFB_OK;
 }
 

@@ -143,6 +143,33 @@ __global__ void __launch_bounds__(1024) seg_compact_kernel(int n_seg, const int 
     }
 }
 
+// 8-bit cache: the segments' rows as dfb_kv_append and dfb_kv_attention want them, one dense array.
+__global__ void seg_row_off_kernel(int n_seg, const int *seg_cnt, const int *cnt, int32_t *row_off) {
+    for (int s = threadIdx.x; s <= n_seg; s += blockDim.x) row_off[s] = s < n_seg ? seg_cnt[s * SEG_N + SEG_AOFF] : cnt[CNT_M];
+}
+// The active rows of Q in f16 (the attention's operand type), and its f16 output rows as the O
+// projection's pair rows (n a multiple of 64).  Bound: latency (a few MB); one block a row.
+__global__ void __launch_bounds__(256) rows_half_kernel(const float *__restrict__ q, int n, const int *__restrict__ cnt, __half *__restrict__ out) {
+    const int a = blockIdx.x;
+    if (a >= cnt[CNT_M]) return;
+    for (int i = 4 * threadIdx.x; i < n; i += 4 * blockDim.x) {
+        const float4 v = *reinterpret_cast<const float4 *>(q + (size_t)a * n + i);
+        __half2 *o = reinterpret_cast<__half2 *>(out + (size_t)a * n + i);
+        o[0] = __floats2half2_rn(v.x, v.y);
+        o[1] = __floats2half2_rn(v.z, v.w);
+    }
+}
+__global__ void __launch_bounds__(256) rows_pair_kernel(const __half *__restrict__ in, int n, const int *__restrict__ cnt, uint8_t *__restrict__ out) {
+    const int a = blockIdx.x;
+    if (a >= cnt[CNT_M]) return;
+    for (int i = 4 * threadIdx.x; i < n; i += 4 * blockDim.x) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(in + (size_t)a * n + i);
+        const float2 x = __half22float2(h[0]), y = __half22float2(h[1]);
+        const float v[4] = {x.x, x.y, y.x, y.y};
+        store_pair4(out + (size_t)a * 4 * n, i, v);
+    }
+}
+
 // x[a] = token_embd[seq[active_pos[a]]] as f32 (ggml_get_rows, graph.cpp:43/433).
 template <typename T>
 __global__ void embed_kernel(const T *__restrict__ emb, int d, int n_vocab, const int32_t *__restrict__ seq,

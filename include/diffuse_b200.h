@@ -97,6 +97,14 @@ int  dfb_model_bytes(const dfb_model *m, size_t *bytes);
 int  dfb_ctx_create(dfb_model *m, int n_ctx, dfb_ctx **out);
 void dfb_ctx_free(dfb_ctx *c);
 
+/* Keep the context's K/V between steps (InterStepCache, diffuse-cache.h:14-147) in 8 bits instead of
+ * f32: a quarter of the memory and of the bytes each step's attention reads.  K and V rows are stored
+ * by dfb_kv_append (pages of 64 positions of one sequence), attention is dfb_kv_attention with Q and
+ * the output rounded to f16; everything else is as before.  Stored values are off by up to 1 part in
+ * 16, so logits move by some percent.  Heads of 64 or 128.  A generation in progress is dropped; may
+ * be called with on = 0 to go back. */
+int dfb_ctx_set_kv8(dfb_ctx *c, int on);
+
 /* diffuse_forward (diffuse-graph.cpp:676-680): full forward over n host tokens, logits
  * copied to the host buffer [n * n_vocab]. */
 int dfb_forward(dfb_ctx *c, const int32_t *tokens, int n, float *logits_host);
