@@ -141,15 +141,30 @@ int code_map(CUtensorMap *m, void *codes, const dfb_kv_cache &c) {
 struct AttnPlan {
     int rows, tiles, splits;
 };
+// 16, 32 and 64 rows: mma.sync, two CTAs to an SM; 256: tcgen05, one.  Up to 64 packed rows take the
+// smallest tile.  More take tcgen05 tiles, which pass four times the rows over a key tile in little more
+// time, but start and finish slowly: where 64-row tiles, each with a part of the keys, give no SM more
+// than one CTA and no CTA more than kShortTiles key tiles, they are faster (of one sequence of 256 rows
+// and 32 heads, us: 320 keys 14.0 against 19.9, 768 keys 22.3 against 25.9, 2048 keys 47 against 32; of
+// 32 rows of 28 / 4 heads: 2048 keys 15.7 against 22.4, 8192 keys 30.5 against 26.9).
+// The key axis is split only as far as SMs would be idle, and to no fewer than four key tiles: a part
+// costs its rows' sums a trip through memory (256 rows, 32 heads, 8192 keys in 1, 2, 4, 8 parts: 162,
+// 95, 61, 75 us).
+constexpr int kShortTiles = 12;
 AttnPlan attn_plan(const dfb_kv_cache &c, const dfb_kv_attn &a, int n_sm) {
-    AttnPlan p;
-    const int64_t packed = (int64_t)a.max_rows * (a.n_q / c.n_kv);
-    p.rows = packed <= 16 ? 16 : packed <= 32 ? 32 : packed <= 64 ? 64 : kTcRows;
-    p.tiles = (int)((packed + p.rows - 1) / p.rows);
-    const int64_t base = (int64_t)p.tiles * c.n_kv * c.n_seq, key_tiles = (a.max_keys + kKeyTile - 1) / kKeyTile;
-    const int64_t want = (p.rows == kTcRows ? 1 : 2) * n_sm / std::max<int64_t>(base, 1);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, key_tiles / 4, kMaxSplits}));
-    return p;
+    const int64_t packed = (int64_t)a.max_rows * (a.n_q / c.n_kv), key_tiles = (a.max_keys + kKeyTile - 1) / kKeyTile;
+    auto plan = [&](int rows, int64_t ctas) {
+        AttnPlan p;
+        p.rows = rows;
+        p.tiles = (int)((packed + rows - 1) / rows);
+        const int64_t base = (int64_t)p.tiles * c.n_kv * c.n_seq;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ctas / std::max<int64_t>(base, 1), key_tiles / 4, kMaxSplits}));
+        return p;
+    };
+    if (packed <= 64) return plan(packed <= 16 ? 16 : packed <= 32 ? 32 : 64, 2 * n_sm);
+    const AttnPlan p = plan(64, n_sm);
+    const bool alone = (int64_t)p.tiles * c.n_kv * c.n_seq <= n_sm;
+    return alone && key_tiles <= (int64_t)kShortTiles * p.splits ? p : plan(kTcRows, n_sm);
 }
 size_t attn_ws_bytes(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p) {
     return p.splits == 1 ? 0 : (size_t)p.splits * a.n_rows * a.n_q * (c.head_dim + 1) * sizeof(float);
