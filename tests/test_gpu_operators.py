@@ -469,6 +469,99 @@ def test_attention_bad_device_values(ops):
     assert bool(((out.double() - ref).abs() <= tol).all()) and bool(((lse.double() - rl).abs() <= ltol).all())
 
 
+# Calls of many rows take large row tiles only where many sequences or a large bound of the keys make them
+# pay: the same scenarios with them, the key axis split (a large max_keys) and whole (many sequences).
+FAR = 200_000
+
+
+@pytest.mark.parametrize("split", [True, False], ids=["split", "whole"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("n_kv,n_q,hd,page,lens,counts", [
+    (1, 7, 128, 32, [95, 31, 200], [9, 31, 100]),
+    (3, 3, 128, 128, [129, 1, 384], [129, 1, 17]),
+    (2, 16, 64, 64, [70, 300, 0], [33, 16, 2]),
+    (1, 1, 128, 64, [640], [300]),
+    (1, 32, 64, 16, [1000, 17], [13, 40]),
+    (2, 8, 128, 16, [1, 700], [70, 0]),
+], ids=["gqa7-p32", "mha-p128", "gqa8-hd64", "long-rows", "mqa32-p16", "one-key"])
+def test_attention_large_tiles(ops, split, dtype, n_kv, n_q, hd, page, lens, counts):
+    times = 1 if split else -(-160 // (n_kv * len(lens)))
+    lens, counts = lens * times, counts * times
+    most = max(1, max(-(-m // page) for m in lens))
+    c = kill_tail(make_cache(ops, len(lens), n_kv, hd, page, most, seed=17), lens)
+    q = torch.randn((sum(counts), n_q, hd), generator=gen(12), device="cuda").to(dtype)
+    off = np.cumsum([0] + counts).tolist()
+    bound = FAR if split else max(lens)
+    out, lse = check_attention(ops, c, q, off, lens, max_keys=bound)
+    again = ops.kv_attention(c, q, ints(off), ints(lens), max_rows=max(counts), max_keys=bound, return_lse=True)
+    assert bool((again[0] == out).all()) and bool((again[1] == lse).all())
+
+
+@pytest.mark.parametrize("split", [True, False], ids=["split", "whole"])
+def test_attention_large_tiles_visible_keys(ops, split):
+    g = gen(14)
+    n_seq, rows, keys, n_kv = (2, 150, 1000, 2) if split else (40, 40, 300, 2)
+    lens = [keys - 5 * (i % 2) for i in range(n_seq)]
+    c = kill_tail(make_cache(ops, n_seq, n_kv, 128, 64, -(-keys // 64), seed=11), lens)
+    q = torch.randn((n_seq * rows, 3 * n_kv, 128), generator=g, device="cuda").to(torch.bfloat16)
+    off = [rows * i for i in range(n_seq + 1)]
+    bound = FAR if split else keys
+    check_attention(ops, c, q, off, lens, vis=[m - rows + t + 1 for m in lens for t in range(rows)], max_keys=bound)
+    random = torch.randint(0, keys + 9, (n_seq * rows,), generator=g, device="cuda").tolist()
+    random[0], random[-1] = 0, 1
+    check_attention(ops, c, q, off, lens, vis=random, max_keys=bound)
+    out, lse = ops.kv_attention(c, q, ints(off), ints(lens), max_rows=rows, max_keys=bound, vis=ints([0] * (n_seq * rows)), return_lse=True)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_attention_large_tiles_scales_apart(ops):
+    g, rows, lens = gen(19), 140, [500]
+    c = kill_tail(make_cache(ops, 1, 2, 128, 32, 16, seed=12), lens)
+    c.v_scale.copy_(torch.exp2(torch.randint(-40, 20, c.v_scale.shape, generator=g, device="cuda").float()))
+    c.k_scale.copy_(torch.exp2(torch.randint(-20, -4, c.k_scale.shape, generator=g, device="cuda").float()))
+    q = torch.randn((rows, 4, 128), generator=g, device="cuda").half()
+    for x, scale in ((q, None), (q, -0.3), (q * 2.0**-12, 300.0), (q, 0.0)):
+        check_attention(ops, c, x, [0, rows], lens, scale=scale, max_keys=FAR)
+    big = (torch.randn((rows, 4, 128), generator=g, device="cuda") * 2.0**30).bfloat16()
+    check_attention(ops, c, big, [0, rows], lens, scale=2.0**-33, max_keys=FAR)
+
+
+def test_attention_large_tiles_layouts_and_bad_values(ops):
+    g, n, n_q, hd = gen(20), 70, 4, 128
+    lens = [333]
+    c = kill_tail(make_cache(ops, 1, 2, hd, 64, 6, seed=13), lens)
+    base = torch.randn(n * n_q * (hd + 1) + 9, generator=g, device="cuda").half()
+    q = base.as_strided((n, n_q, hd), (hd + 1, n * (hd + 1), 1), 3)
+    out = torch.full((n_q, n + 2, hd + 3), 7.0, dtype=torch.float16, device="cuda")
+    check_attention(ops, c, q, [0, n], lens, out=out[:, 1 : n + 1, 1 : hd + 1].transpose(0, 1), max_keys=FAR)
+    edge = out.clone()
+    edge[:, 1 : n + 1, 1 : hd + 1] = 7.0
+    assert bool((edge == 7.0).all())
+    q = q.contiguous()
+
+    def run(off, lens, max_rows=n):
+        st = ints([0])
+        out, lse = ops.kv_attention(c, q, ints(off), ints(lens), max_rows=max_rows, max_keys=FAR, return_lse=True, status=st, out=torch.full_like(q, 3.0))
+        return out, lse, int(st)
+
+    assert run([0, n], [400])[2] == ops.STAT_POSITION
+    out, lse, st = run([0, n], [-1])
+    assert st == ops.STAT_POSITION and bool((out == 0).all()) and bool((lse == -math.inf).all())
+    out, _, st = run([40, 20], [333])
+    assert st == ops.STAT_ROWS and bool((out == 3.0).all())
+    out, _, st = run([0, n], [333], max_rows=50)
+    assert st == ops.STAT_ROWS and bool((out[50:] == 3.0).all())
+    pages = c.pages.clone()
+    bad = pages.clone()
+    bad[0, 1] = -1
+    c.set_pages(bad)
+    out, lse, st = run([0, n], [320])
+    assert st == ops.STAT_PAGE
+    c.set_pages(pages[:, [0, 2, 3, 4]].contiguous())
+    ref, rl, tol, ltol = ref_attention(c, q, [0, n], [256], None, hd**-0.5)
+    assert bool(((out.double() - ref).abs() <= tol).all()) and bool(((lse.double() - rl).abs() <= ltol).all())
+
+
 # ── log probabilities ──
 
 
