@@ -26,7 +26,7 @@
 
 namespace dfb {
 
-constexpr int kLpThreads = 256, kLpCtas = 4 /* of an SM */, kLpWarps = kLpThreads / 32, kLpMaxK = 32, kLpCap = 4096;
+constexpr int kLpThreads = 256, kLpCtas = 4 /* of an SM */, kLpWarps = kLpThreads / 32, kLpMaxK = 32, kLpCap = 4096, kLpFew = 256;
 constexpr float kLpLn2 = 0.6931471805599453f, kLpLog2e = 1.4426950408889634f, kLpFloor = -200.f;
 
 struct LpSmem {
@@ -35,7 +35,7 @@ struct LpSmem {
     unsigned long long group[32];
     float m[kLpWarps], z[kLpWarps], t[kLpWarps];
     float part[3];                        // this CTA's m, z, t
-    int count, n_top;
+    int count, n_top, kept;
 };
 
 __device__ __forceinline__ unsigned long long lp_key(float x, int id) {
@@ -124,13 +124,55 @@ __device__ __forceinline__ void lp_push(LpSmem &s, unsigned long long key) {
     const int at = atomicAdd(&s.count, 1);
     if (at < kLpCap) s.list[at] = key;
 }
-// The k largest of n keys (n >= 0, all different) to top, in order; every thread of the block takes part.
-__device__ __forceinline__ void lp_rank(const unsigned long long *list, int n, unsigned long long *top, int k) {
-    for (int i = threadIdx.x; i < n; i += kLpThreads) {
-        const unsigned long long key = list[i];
+// With mine the largest key of group `lane` (32 groups of one set): the k-th largest of them, no larger
+// than the set's k-th key (0: fewer than k groups have one).  first: the largest.
+__device__ __forceinline__ unsigned long long lp_kth_group(const LpSmem &s, int k, unsigned long long *first = nullptr) {
+    const int lane = threadIdx.x & 31;
+    const unsigned long long mine = s.group[lane];
+    int r = 0;
+#pragma unroll
+    for (int j = 0; j < 32; j++) {
+        const unsigned long long c = s.group[j];
+        r += c > mine || (c == mine && j < lane);
+    }
+    if (first) *first = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, r == 0)) - 1);
+    return k > 0 ? __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, r == k - 1)) - 1) : 0;
+}
+// A group is eight threads: each gives its largest key.
+__device__ __forceinline__ void lp_group_max(LpSmem &s, unsigned long long key) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+        const unsigned long long c = __shfl_xor_sync(0xffffffffu, key, o);
+        key = c > key ? c : key;
+    }
+    if ((threadIdx.x & 7) == 0) s.group[threadIdx.x >> 3] = key;
+}
+// The k largest of the list's n keys (n >= 0, all different) to s.top, in order; every thread of the block
+// takes part, and the list is used up.  Counting each key's betters is n^2 steps (3151 keys: 300 us), so
+// more than kLpFew of them are first held against the k-th of 32 groups' largest, which leaves some 4 k.
+__device__ __forceinline__ void lp_rank(LpSmem &s, int n, int k) {
+    const int tid = threadIdx.x;
+    for (int pass = 0; n > kLpFew && pass < 4; pass++) {
+        unsigned long long key = 0;
+        for (int i = tid; i < n; i += kLpThreads) key = s.list[i] > key ? s.list[i] : key;
+        lp_group_max(s, key);
+        if (tid == 0) s.kept = 0;
+        __syncthreads();
+        const unsigned long long thr = lp_kth_group(s, k);
+        for (int i0 = 0; i0 < n; i0 += kLpThreads) {
+            key = i0 + tid < n ? s.list[i0 + tid] : 0;
+            __syncthreads();  // (what is kept goes to places that have been read)
+            if (key && key >= thr) s.list[atomicAdd(&s.kept, 1)] = key;
+        }
+        __syncthreads();
+        n = s.kept;
+        __syncthreads();
+    }
+    for (int i = tid; i < n; i += kLpThreads) {
+        const unsigned long long key = s.list[i];
         int r = 0;
-        for (int j = 0; j < n; j++) r += list[j] > key;
-        if (r < k) top[r] = key;
+        for (int j = 0; j < n; j++) r += s.list[j] > key;
+        if (r < k) s.top[r] = key;
     }
 }
 
@@ -239,7 +281,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
         const int n = s.count;
         __syncthreads();  // (no one adds to it before all have read it)
         if (n < k || n > kLpCap) return;
-        lp_rank(s.list, n, s.top, k);
+        lp_rank(s, n, k);
         __syncthreads();
         if (tid < k) s.list[tid] = s.top[tid];
         if (tid == 0) s.count = k;
@@ -262,27 +304,12 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
                 const unsigned long long c = lp_key(bm, id_of(0, e));
                 key = c > key ? c : key;
             }
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-            const unsigned long long c = __shfl_xor_sync(0xffffffffu, key, o);
-            key = c > key ? c : key;
-        }
-        if ((lane & 7) == 0) s.group[tid >> 3] = key;
+        lp_group_max(s, key);
         __syncthreads();
-        const unsigned long long mine = s.group[lane];  // every warp finds the same
-        int r = 0;
-#pragma unroll
-        for (int j = 0; j < 32; j++) {
-            const unsigned long long c = s.group[j];
-            r += c > mine || (c == mine && j < lane);
-        }
-        const unsigned first = __ballot_sync(0xffffffffu, r == 0), kth = __ballot_sync(0xffffffffu, r == k - 1);
-        const unsigned long long best = __shfl_sync(0xffffffffu, mine, __ffs(first) - 1);
+        unsigned long long best;
+        thr = lp_kth_group(s, k, &best);  // (every warp finds the same)
         if (best) sum.m = lp_value(best);
-        if (k > 0 && v1 - v0 > kLpCap / B::PER) {
-            thr = __shfl_sync(0xffffffffu, mine, __ffs(kth) - 1);
-            thr_x = thr ? lp_value(thr) : -INFINITY;
-        }
+        if (thr) thr_x = lp_value(thr);
         add(cur, bm);
         if (k > 0) look(cur, 0, bm);
     }
@@ -362,7 +389,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
         }
         __syncthreads();
         const int n = min(s.count, kLpCap);
-        lp_rank(s.list, n, s.top, k);
+        lp_rank(s, n, k);
         if (tid == 0) s.n_top = min(n, k);
     }
     // ── the cluster's: the first CTA takes the others' ──
@@ -398,7 +425,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
             __syncthreads();
             if (key) s.list[atomicAdd(&s.count, 1)] = key;
             __syncthreads();
-            lp_rank(s.list, s.count, s.top, k);
+            lp_rank(s, s.count, k);
             if (tid == 0) s.n_top = min(s.count, k);
         }
     } else if (tid == 0) {
