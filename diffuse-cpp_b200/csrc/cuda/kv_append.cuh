@@ -192,10 +192,14 @@ __device__ __forceinline__ uint2 encode8(const float2 *v, float f) {
 // its values between the maximum and the conversion, and the next head's rows as they come, so rows are
 // read once and the table's rows once for a group of heads.
 //
-// Bound: memory (rows in, codes out), if the rotation is cheap: rot_odd's sixteen instructions a value
-// took 520 us for 32768 rows of 32 + 32 + 32 heads.  rot_near's four decide every code but those whose
-// value lies within kRotTol of a border of two codes (one in 10^5), and the scale unless the maximum
-// lies that near to 448 * 2^e; those are worked out again with rot_odd.
+// Bound: memory (rows in, codes out) as long as the rotation is cheap: rot_odd takes sixteen instructions
+// a value.  rot_near's four, for two values at a time, decide every code but those whose value lies within
+// kRotTol of a border of two codes (one in 10^5), and the scale unless the maximum lies that near to
+// 448 * 2^e; those are worked out again with rot_odd, from memory, so that the usual path keeps its
+// registers.  bf16, 32768 rows of 32 + 32 + 32 heads of 128, pages of 64: 321 us, 4.2 TB/s (520 us with
+// scalar arithmetic and rows loaded when they are due); f32, 4096 rows: 76 us, 4.0 TB/s.  What is left is
+// half issue slots (15 instructions a value in all), half the barrier each head's maximum needs.  Rows
+// three heads ahead through shared memory gave 314 us, and 95 us for f32: not worth their memory.
 template <typename T, int HD, int kAppendThreads>
 __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 1024 || sizeof(T) == 2 ? 1024 / kAppendThreads : 512 / kAppendThreads) kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, int heads, bool vec,
                                                                       int32_t *status) {

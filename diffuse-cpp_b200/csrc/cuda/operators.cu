@@ -104,7 +104,7 @@ int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, int64_t pages, int n_s
     const int64_t filled = std::min<int64_t>(pages * c.n_seq, r.n_rows / c.page + c.n_seq);  // pages with rows, about
     while (heads > 1 && filled * blocks_y() < 4 * n_sm) heads /= 2;
     const dim3 grid((unsigned)pages, blocks_y(), c.n_seq);
-    const int items = c.page * (HD / 16);
+    const int items = c.page * (HD / 16);  // of a page: one thread each
     if (items <= 256) kv_append_kernel<T, HD, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
     else if (items <= 512) kv_append_kernel<T, HD, 512><<<grid, 512, 0, st>>>(c, r, heads, vec, status);
     else kv_append_kernel<T, HD, 1024><<<grid, 1024, 0, st>>>(c, r, heads, vec, status);
