@@ -783,7 +783,6 @@ struct dfb_ctx {
     // dfb_score: the alternatives of each position
     int32_t *score_ids = nullptr;
     float *score_lp = nullptr;
-    int score_cap = 0;
     // generation
     bool gen_active = false;
     int total = 0;                   // positions of all segments
@@ -807,7 +806,6 @@ static void ctx_free_buffers(dfb_ctx *c) {
     c->kv8.on = kv8_on;
     c->score_ids = nullptr;
     c->score_lp = nullptr;
-    c->score_cap = 0;
     c->seg_off = c->seg_cnt = c->sched = c->tmp_active = c->tmp_masked = c->rope_pos = c->masked_row = nullptr;
     c->done = nullptr;
     c->tiles = nullptr;
@@ -851,6 +849,7 @@ static int ctx_reserve(dfb_ctx *c, int n) {
     AL(c->seq, cap); AL(c->prev_seq, cap); AL(c->last_changed, cap); AL(c->cand_tok, cap); AL(c->commit_pos, cap);
     AL(c->commit_tok, cap); AL(c->order, cap); AL(c->masked, cap); AL(c->active_pos, cap); AL(c->masked_pos, cap);
     AL(c->cnt, CNT_N); AL(c->cand_conf, cap); AL(c->cand_ent, cap); AL(c->unif, cap);
+    AL(c->score_ids, (size_t)cap * kScoreTop); AL(c->score_lp, (size_t)cap * kScoreTop);
     if (m->tp_size > 1) { AL(c->tp_stats, cap); AL(c->tp_gath, (size_t)cap * m->tp_size); AL(c->tp_g, cap); }
     AL(c->seg_off, kMaxSeg + 1); AL(c->seg_cnt, kMaxSeg * SEG_N); AL(c->sched, kMaxSeg); AL(c->done, kMaxSeg);
     AL(c->tmp_active, cap); AL(c->tmp_masked, cap); AL(c->rope_pos, cap); AL(c->masked_row, cap);
@@ -1433,16 +1432,6 @@ extern "C" int dfb_score(dfb_ctx *c, const int32_t *tokens, int n, const int32_t
     for (int i = 0; i < n; i++) rows[i] = m->hp.shift_logits && i > 0 ? i - 1 : i;
     std::lock_guard<std::mutex> lk(device_lock(m->device));
     RET(forward_tokens(c, tokens, n));
-    if (top_k && c->score_cap < c->cap) {
-        cudaFree(c->score_ids);
-        cudaFree(c->score_lp);
-        c->score_ids = nullptr;
-        c->score_lp = nullptr;
-        c->score_cap = 0;
-        CK(cudaMalloc(&c->score_ids, (size_t)c->cap * kScoreTop * sizeof(int32_t)));
-        CK(cudaMalloc(&c->score_lp, (size_t)c->cap * kScoreTop * sizeof(float)));
-        c->score_cap = c->cap;
-    }
     dfb_logprob_args a{};
     a.logits = c->logits;
     a.type = G_F32;
@@ -1460,7 +1449,11 @@ extern "C" int dfb_score(dfb_ctx *c, const int32_t *tokens, int n, const int32_t
     a.top_k = top_k;
     a.top_ids = c->score_ids;
     a.top_logprob = c->score_lp;
-    RET(dfb_token_logprobs(&a, nullptr, c->st));
+    const int rc = dfb_token_logprobs(&a, nullptr, c->st);
+    if (rc != DFB_OK) {
+        cudaStreamSynchronize(c->st);  // (the forward's GEMMs end before the device lock is given back)
+        return rc;
+    }
     auto fetch = [&](void *dst, const void *src, size_t count) {
         return dst && count ? cudaMemcpyAsync(dst, src, count * 4, cudaMemcpyDeviceToHost, c->st) : cudaSuccess;
     };

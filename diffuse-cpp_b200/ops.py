@@ -68,6 +68,14 @@ def _stream(index, stream):
     return torch._C._cuda_getCurrentRawStream(index) if stream is None else stream
 
 
+def _empty(like, shape, dtype, index, stream):
+    """A new tensor whose memory goes back to the stream that the call runs on."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=index)):
+        return like.new_empty(shape, dtype=dtype)
+
+
 # (device indices are compared as integers: a call's checks take a few microseconds, and its kernel may not
 # take more)
 def _ints(name, t, index, n=None):
@@ -179,11 +187,11 @@ def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: i
     n, n_q, hd = q.shape
     sq = _rows("q", q, q.dtype, d, (n, n_q, cache.head_dim))
     if out is None:
-        out = q.new_empty((n, n_q, hd))
+        out = _empty(q, (n, n_q, hd), q.dtype, d, stream)
         so = (n_q * hd, hd)
     else:
         so = _rows("out", out, q.dtype, d, (n, n_q, hd))
-    lse = q.new_empty((n, n_q), dtype=torch.float32) if return_lse else None
+    lse = _empty(q, (n, n_q), torch.float32, d, stream) if return_lse else None
     a = _KvAttn(q.data_ptr(), out.data_ptr(), typ, n_q, n, max_rows, max_keys, hd**-0.5 if scale is None else scale, sq[0], sq[1],
                 so[0], so[1], _ints("row_off", row_off, d, cache._n_seq + 1), _ints("lens", lens, d, cache._n_seq),
                 _ints("vis", vis, d, n), None if lse is None else lse.data_ptr())
@@ -193,7 +201,7 @@ def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: i
             need = cache._ws[n_q, n, max_rows, max_keys] = kv_attention_workspace(cache, n_q=n_q, n_rows=n, max_rows=max_rows,
                                                                                   max_keys=max_keys)
         if need:
-            workspace = q.new_empty((need,), dtype=torch.uint8)
+            workspace = _empty(q, (need,), torch.uint8, d, stream)
     elif workspace.get_device() != d or not workspace.is_contiguous():
         raise ValueError(f"workspace must be a contiguous tensor on {cache.device}")
     _ck(_fn("dfb_kv_attention")(cache._ref, C.addressof(a), None if workspace is None else workspace.data_ptr(),
@@ -224,7 +232,7 @@ def token_logprobs(logits, targets=None, *, top_k: int = 0, rows=None, status=No
     k = max(top_k, 0)
     tp = _ints("targets", targets, d, n)
     # one allocation: logprob, entropy, top_logprob, then the ids
-    lp, ent, top, ids = logits.new_empty((n * (2 + 2 * k),), dtype=torch.float32).split((n, n, n * k, n * k))
+    lp, ent, top, ids = _empty(logits, (n * (2 + 2 * k),), torch.float32, d, stream).split((n, n, n * k, n * k))
     top, ids = top.view(n, k), ids.view(torch.int32).view(n, k)
     a = _Logprobs(logits.data_ptr(), _TYPES[logits.dtype], v, n, logits.shape[0], logits.stride(0), _ints("rows", rows, d), tp,
                   lp.data_ptr() if tp else None, ent.data_ptr(), top_k, ids.data_ptr() if k else None, top.data_ptr() if k else None)

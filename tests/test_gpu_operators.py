@@ -562,6 +562,35 @@ def test_attention_large_tiles_layouts_and_bad_values(ops):
     assert bool(((out.double() - ref).abs() <= tol).all()) and bool(((lse.double() - rl).abs() <= ltol).all())
 
 
+def test_attention_no_keys_at_all(ops):
+    for rows, bound in ((3, 0), (90, 0), (90, FAR)):
+        c = make_cache(ops, 2, 2, 64, 16, 2, seed=21)
+        q = torch.randn((2 * rows, 4, 64), generator=gen(22), device="cuda").half()
+        out, lse = ops.kv_attention(c, q, ints([0, rows, 2 * rows]), ints([0, 0]), max_rows=rows, max_keys=bound, return_lse=True)
+        assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_outputs_and_workspace_on_a_given_stream(ops):
+    """Memory that a call allocates belongs to the stream it runs on: work on the current stream right after
+    the call may not be given its workspace."""
+    side = torch.cuda.Stream()
+    lens, rows = [20000], 64
+    c = kill_tail(make_cache(ops, 1, 2, 128, 64, 313, seed=23), lens)
+    q = torch.randn((rows, 4, 128), generator=gen(24), device="cuda").half()
+    off, ln = ints([0, rows]), ints(lens)
+    x = torch.randn((40, 30000), generator=gen(25), device="cuda")
+    want = ops.kv_attention(c, q, off, ln, max_rows=rows, max_keys=20000)
+    ref = ops.token_logprobs(x, top_k=9)
+    torch.cuda.synchronize()
+    need = ops.kv_attention_workspace(c, n_q=4, n_rows=rows, max_rows=rows, max_keys=20000)
+    for _ in range(20):
+        got = ops.kv_attention(c, q, off, ln, max_rows=rows, max_keys=20000, stream=side.cuda_stream)
+        lp = ops.token_logprobs(x, top_k=9, stream=side.cuda_stream)
+        torch.empty(need, dtype=torch.uint8, device="cuda").fill_(0xFF)
+        side.synchronize()
+        assert bool((got == want).all()) and bool((lp[1] == ref[1]).all()) and bool((lp[2] == ref[2]).all())
+
+
 # ── log probabilities ──
 
 
