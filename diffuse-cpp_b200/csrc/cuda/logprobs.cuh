@@ -15,9 +15,9 @@
 //
 // Bound: the row read once from memory, and issue slots beside it: four instructions and one ex2 a value,
 // one more for the batch's largest, two more where alternatives are wanted.  2048 rows of 152064 bf16:
-// 186 us, 3.3 TB/s (138 us without alternatives); 256 rows of 126464 f32: 35 us, 3.7 TB/s (27).  A row is
+// 176 us, 3.5 TB/s (138 us without alternatives); 256 rows of 126464 f32: 32 us, 4.0 TB/s (27).  A row is
 // split over the CTAs of a cluster (joined through distributed shared memory) where rows alone would leave
-// SMs without work: one row of 126464 in 8 CTAs takes 17 us, of which 5 are launch and first batch.
+// SMs without work: one row of 126464 in 8 CTAs takes 12 us, of which 5 are launch and first batch.
 #pragma once
 #include <cstdint>
 #include <type_traits>
@@ -265,6 +265,11 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
         uint32_t pass = 0;
 #pragma unroll
         for (int e = 0; e < B::N; e++) pass |= b.at(e) >= least ? 1u << e : 0u;
+        if ((pass & (pass - 1)) == 0) {  // the usual case: it is the largest (2048 rows 176 us, with the loop alone 180)
+            const unsigned long long key = lp_key(bm, id_of(r, __ffs(pass) - 1));
+            if (pass && key >= thr) lp_push(s, key);
+            return;
+        }
         while (pass) {
             const int e = __ffs(pass) - 1;
             pass &= pass - 1;
@@ -325,14 +330,13 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
         if (k > 0) look1(x_tail, tail + tid);
     }
     // a threshold from n of the row's elements lets some k (row / n - 1) more pass: it is taken again after
-    // 1, 4, 13, ... batches (taken once, 2048 rows of 152064 with k = 20 took 282 us, most
-    // of them for what it let pass)
+    // 1, 3, 7, ... batches (2048 rows of 152064 with k = 20: 180 us, after 1, 4, 13, ... 184, 1, 6, 31 208, once 332)
     int again = 1;
     auto batch = [&](const B &b, B &spare, int r) {
         load(spare, r + 1);
         if (k > 0 && r == again) {
             tighten();
-            again = 3 * again + 1;
+            again = 2 * again + 1;
         }
         const float bm = largest(b);
         add(b, bm);
