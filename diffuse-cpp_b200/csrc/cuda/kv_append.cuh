@@ -29,42 +29,6 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive elements as f32; vec: 16-byte loads are aligned.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4 *>(p);
-            const T *t = reinterpret_cast<const T *>(&u);
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = to_f32<T>(t[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = to_f32<T>(p[i]);
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T *p, bool vec, const float (&v)[8]) {
-    T t[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) t[i] = from_f32<T>(v[i]);
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(t);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) p[i] = t[i];
-    }
-}
-
 // Two consecutive elements as f32, and back.
 template <typename T>
 __device__ __forceinline__ float2 pair_at(const uint4 *v, int e) {
@@ -197,12 +161,17 @@ __device__ __forceinline__ uint2 encode8(const float2 *v, float f) {
 // kRotTol of a border of two codes (one in 10^5), and the scale unless the maximum lies that near to
 // 448 * 2^e; those are worked out again with rot_odd, from memory, so that the usual path keeps its
 // registers.  bf16, 32768 rows of 32 + 32 + 32 heads of 128, pages of 64: 321 us, 4.2 TB/s (520 us with
-// scalar arithmetic and rows loaded when they are due); f32, 4096 rows: 76 us, 4.0 TB/s.  What is left is
-// half issue slots (15 instructions a value in all), half the barrier each head's maximum needs.  Rows
+// scalar arithmetic and rows loaded when they are due); f32, 4096 rows: 75 us, 4.0 TB/s.  What is left is
+// the wait for a head's rows and for its maximum (the barrier); half the issue slots are idle.  Rows
 // three heads ahead through shared memory gave 314 us, and 95 us for f32: not worth their memory.
+// 1024 threads of an SM with 64 registers each; f32 rows, twice as long, 512 with 128 where a page allows
+// (4096 rows: 75 us, with 1024 and spills 82).
+template <typename T, int N>
+constexpr int kAppendCtas = (sizeof(T) == 2 || N == 1024 ? 1024 : 512) / N;
+
 template <typename T, int HD, int kAppendThreads>
-__global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 1024 || sizeof(T) == 2 ? 1024 / kAppendThreads : 512 / kAppendThreads) kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, int heads, bool vec,
-                                                                      int32_t *status) {
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T, kAppendThreads>)
+    kv_append_kernel(const dfb_kv_cache c, const dfb_kv_rows r, int heads, bool vec, int32_t *status) {
     constexpr int IPR = HD / 16;  // items per row
     __shared__ uint32_t red[3];
     __shared__ uint32_t written[4];
@@ -353,7 +322,8 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 1024 || size
             }
         }
         amax = block_max(amax, head - head0);
-        if (rotate && need_exp(amax * (1.f - kRotTol)) != need_exp(amax * (1.f + kRotTol))) {  // (the same for the whole block)
+        int e = need_exp(rotate ? amax * (1.f + kRotTol) : amax);
+        if (rotate && e > -64 && amax * (1.f - kRotTol) <= 448.f * exp2i(e - 1)) {  // (the same for the whole block)
             amax = 0.f;
             if (slot >= 0) {
 #pragma unroll 1
@@ -366,9 +336,8 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendThreads == 1024 || size
             __syncthreads();
             if (tid == 0) red[(head - head0) % 3] = 0;
             __syncthreads();
-            amax = block_max(amax, head - head0);
+            e = need_exp(block_max(amax, head - head0));
         }
-        int e = need_exp(amax);
         if (survive) {
             if (old >= e) e = old;
             else {  // grown: re-round the kept codes

@@ -105,6 +105,42 @@ constexpr int kKvStages = 4;
 
 constexpr int kMaxSplits = 128;
 
+// Eight consecutive elements as f32; vec: 16-byte loads are aligned.
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, bool vec, float (&v)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4 *>(p);
+            const T *t = reinterpret_cast<const T *>(&u);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = to_f32<T>(t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32<T>(p[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T *p, bool vec, const float (&v)[8]) {
+    T t[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) t[i] = from_f32<T>(v[i]);
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4 *>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(t);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = t[i];
+    }
+}
+
 // Where a call's split parts go: normalised rows and their log2 weights, [split][row][query head].
 struct AttnParts {
     float *o = nullptr;    // [splits][n_rows * n_q][head_dim]
