@@ -22,6 +22,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -1367,7 +1368,11 @@ static int set_segments(dfb_ctx *c, const std::vector<int> &off) {
     c->n_seg = n;
     c->seg_off_h = off;
     c->total = off.back();
-    return c->kv8.on ? kv8_layout(c) : DFB_OK;
+    try {
+        return c->kv8.on ? kv8_layout(c) : DFB_OK;
+    } catch (const std::bad_alloc &) {
+        return set_err(DFB_ERR_NOMEM, "no host memory for a page table");
+    }
 }
 
 // Active sets and work lists of one step over all segments (seg_prepare + seg_compact).
@@ -1428,7 +1433,12 @@ extern "C" int dfb_score(dfb_ctx *c, const int32_t *tokens, int n, const int32_t
         return set_err(DFB_ERR_ARG, "top_k %d outside [0, %d], or without outputs", top_k, std::min(kScoreTop, m->hp.n_vocab));
     for (int i = 0; targets && i < n; i++)
         if (targets[i] >= m->hp.n_vocab) return set_err(DFB_ERR_ARG, "target %d at %d outside the vocabulary", targets[i], i);
-    std::vector<int32_t> rows(n);  // the logits row that predicts position i: a shifted model's is the one before
+    std::vector<int32_t> rows;  // the logits row that predicts position i: a shifted model's is the one before
+    try {
+        rows.resize(n);
+    } catch (const std::bad_alloc &) {
+        return set_err(DFB_ERR_NOMEM, "no host memory for %d rows", n);
+    }
     for (int i = 0; i < n; i++) rows[i] = m->hp.shift_logits && i > 0 ? i - 1 : i;
     std::lock_guard<std::mutex> lk(device_lock(m->device));
     RET(forward_tokens(c, tokens, n));

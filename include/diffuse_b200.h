@@ -239,7 +239,7 @@ enum {
     DFB_STAT_POSITION = 2,  /* a position outside the page table or the rotation table, or not
                                ascending: its row was left out; a length outside the page table */
     DFB_STAT_ROWS = 4,      /* row_off not ascending within [0, n_rows], or more rows than max_rows */
-    DFB_STAT_NONFINITE = 8, /* K / V to be stored held NaN (stored as 0) or +-inf (stored as the largest code) */
+    DFB_STAT_NONFINITE = 8, /* K / V to be stored held NaN (stored as 0) or +-inf (the largest code); K rotated: either */
     DFB_STAT_TARGET = 16,   /* a target token >= n_vocab (its log probability is NaN), or a row index out of range */
     DFB_STAT_TIMEOUT = 64,  /* a kernel gave up a bounded wait: the outputs are invalid */
     DFB_STAT_LOGITS = 32    /* a logits row with NaN or +inf (its outputs are NaN, its ids -1) */
