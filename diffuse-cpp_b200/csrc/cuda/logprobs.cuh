@@ -67,17 +67,22 @@ __device__ __forceinline__ unsigned long long ld_cluster_u64(const unsigned long
     return v;
 }
 
-// Sums relative to 2^b, b = m log2(e) rounded: y = x log2(e) - b is one fused multiply-add.  With
-// d = m log2(e) - b the sum relative to m is z 2^-d, and b's rounding leaves ln z + ln 2 t / z as it is.
-// Beside f32's largest values the products overflow: y comes from x - m there (b = 0 stands for it).
+// Sums relative to 2^b, b = m log2(e) rounded: y = x log2(e) - b is one fused multiply-add.  With the
+// offset d = m log2(e) - b the sum relative to m is z 2^-d, and b's rounding leaves ln z + ln 2 t / z as it
+// is.  d is up to half a unit in the last place of b, so this holds up to kLpNarrow only, where |d| <= 2^-4;
+// a larger m (a row or a part of one filled with -1e10, say) would send 2^d out of f32's range.  There
+// y = (x - m) log2(e) and d = 0.
+constexpr float kLpNarrow = 1048576.f;  // 2^20
 struct LpSum {
     float m = -3.402823466e38f, z = 0.f, t = 0.f;  // (z = 0: nothing but -inf so far)
-    __device__ __forceinline__ static bool wide(float m) { return fabsf(m) > 1e38f; }
-    __device__ __forceinline__ static float base(float m) { return wide(m) ? 0.f : m * kLpLog2e; }
+    __device__ __forceinline__ static bool wide(float m) { return fabsf(m) > kLpNarrow; }
+    // (a product that the compiler may not fuse with the subtraction that follows it: b is a rounded value)
+    __device__ __forceinline__ static float base(float m) { return __fmul_rn(m, kLpLog2e); }
+    __device__ __forceinline__ static float offset(float m) { return wide(m) ? 0.f : fmaf(m, kLpLog2e, -base(m)); }
     // log2 of what a sum relative to `from` is worth relative to `to` (to >= from)
     __device__ __forceinline__ static float shift(float from, float to) {
         if (from == to) return 0.f;
-        if (wide(from) || wide(to)) return max_nan((from - to) * kLpLog2e, kLpFloor);
+        if (wide(from) || wide(to)) return max_nan(fmaf(from - to, kLpLog2e, offset(to) - offset(from)), kLpFloor);
         return max_nan(base(from) - base(to), kLpFloor);
     }
     __device__ __forceinline__ void raise(float mn) {  // mn >= m
@@ -93,8 +98,7 @@ struct LpSum {
         t += o.t;
     }
     __device__ __forceinline__ float log_z() const {  // ln of the sum relative to m
-        const float d = wide(m) ? 0.f : fmaf(m, kLpLog2e, -base(m));
-        return fmaf(-d, kLpLn2, logf(z));
+        return fmaf(-offset(m), kLpLn2, logf(z));
     }
     __device__ __forceinline__ float entropy() const { return fmaf(t / z, kLpLn2, logf(z)); }
     __device__ __forceinline__ void add1(float f) {
@@ -230,25 +234,27 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
     const float x_head = has_head ? to_f32<T>(x[tid]) : -INFINITY, x_tail = has_tail ? to_f32<T>(x[tail + tid]) : -INFINITY;
     auto add = [&](const B &b, float bm) {
         if (bm > sum.m) sum.raise(bm);
-        if (LpSum::wide(sum.m)) {
-#pragma unroll 1
-            for (int e = 0; e < B::N; e++) {
-                float f = 0.f;
-#pragma unroll
-                for (int c = 0; c < B::N; c++) f = c == e ? b.at(c) : f;
-                sum.add1(f);
-            }
-            return;
-        }
-        const float nb = -LpSum::base(sum.m);
         float2 z = make_float2(0.f, 0.f), t = z;  // t: of y 2^y
-#pragma unroll
-        for (int e = 0; e < B::N; e += 2) {
-            float2 y = fma2(make_float2(b.at(e), b.at(e + 1)), make_float2(kLpLog2e, kLpLog2e), make_float2(nb, nb));
+        auto term = [&](float2 y) {
             y = make_float2(max_nan(y.x, kLpFloor), max_nan(y.y, kLpFloor));
             const float2 p = make_float2(ex2(y.x), ex2(y.y));
             z = add2(z, p);
             t = fma2(y, p, t);
+        };
+        const float2 l2e = make_float2(kLpLog2e, kLpLog2e);
+        if (LpSum::wide(sum.m)) {
+            const float2 nm = make_float2(-sum.m, -sum.m);
+#pragma unroll 1  // (unrolled it costs the usual rows beside it 2 %)
+            for (int e = 0; e < B::N; e += 2) {
+                float2 f = make_float2(b.at(0), b.at(1));
+#pragma unroll
+                for (int c = 2; c < B::N; c += 2) f = c == e ? make_float2(b.at(c), b.at(c + 1)) : f;
+                term(mul2(add2(f, nm), l2e));
+            }
+        } else {
+            const float nb = -LpSum::base(sum.m);
+#pragma unroll
+            for (int e = 0; e < B::N; e += 2) term(fma2(make_float2(b.at(e), b.at(e + 1)), l2e, make_float2(nb, nb)));
         }
         sum.z += z.x + z.y;
         sum.t -= t.x + t.y;
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
     sum.m = s.part[0]; sum.z = s.part[1]; sum.t = s.part[2];
     const float m = sum.m, z = sum.z, lz = sum.log_z();
     const bool bad = !there || z != z, none = z == 0.f;  // NaN or +inf; nothing but -inf
-        auto lp = [&](float f) { return bad ? NAN : none ? -INFINITY : (f - m) - lz; };
+    auto lp = [&](float f) { return bad ? NAN : none ? -INFINITY : (f - m) - lz; };
     if (tid == 0) {
         if (!there) flag(DFB_STAT_TARGET);
         else if (bad) flag(DFB_STAT_LOGITS);
