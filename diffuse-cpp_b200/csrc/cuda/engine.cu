@@ -1175,17 +1175,6 @@ static int tp_sum_rows(dfb_ctx *c) {
     return DFB_OK;
 }
 
-// The value checks of the forward and the sampler (cnt[CNT_ERR]): a token id outside the
-// vocabulary reached the embedding (1), or a logits row had no finite maximum (2).  Reported
-// once and cleared; the kernels read a valid row instead, so nothing faults.
-static int check_values(dfb_ctx *c, int code) {
-    if (!code) return DFB_OK;
-    CK(cudaMemsetAsync(c->cnt + CNT_ERR, 0, sizeof(int), c->st));
-    CK(cudaStreamSynchronize(c->st));
-    return set_err(DFB_ERR_STATE, code == 1 ? "a token id outside the vocabulary reached the embedding"
-                                            : "a logits row has no finite maximum (non-finite logits)");
-}
-
 // The forward of one step over the active rows listed by step_prepare.
 static int run_forward(dfb_ctx *c, int n_total) {
     const dfb_model *m = c->m;
@@ -1273,23 +1262,29 @@ static const char *gemm_err_str(int code) {
 static std::mutex g_device_mu[64];
 static std::mutex &device_lock(int device) { return g_device_mu[device & 63]; }
 
-static int check_err(dfb_ctx *c) {
-    int e = 0;
-    if (c->kv8.on) {
-        CK(cudaMemcpy(&e, c->kv8.status, sizeof(int), cudaMemcpyDeviceToHost));
-        if (e) {
-            cudaMemset(c->kv8.status, 0, sizeof(int));
-            if (e & DFB_STAT_TIMEOUT) return set_err(DFB_ERR_TIMEOUT, "attention over the 8-bit cache stopped; results of this call are invalid");
-            return set_err(DFB_ERR_ARG, "8-bit cache: %s (status %d)", e & DFB_STAT_NONFINITE ? "K or V not finite" : "bad rows", e);
-        }
+// What the device recorded during a call whose work has ended.  All of it is cleared at once, so no later
+// call reports it; time-outs come first, since they leave every other value of the call undefined.
+// values: the forward's and the sampler's checks (cnt[CNT_ERR]), a token id outside the vocabulary at the
+// embedding (1) or a logits row without a finite maximum (2); the kernels read a valid row instead, so
+// nothing faults.
+static int check_err(dfb_ctx *c, int values = 0) {
+    int gemm = 0, kv8 = 0;
+    CK(cudaMemcpy(&gemm, c->err, sizeof(int), cudaMemcpyDeviceToHost));
+    if (c->kv8.on) CK(cudaMemcpy(&kv8, c->kv8.status, sizeof(int), cudaMemcpyDeviceToHost));
+    if (gemm) {
+        CK(cudaMemsetAsync(c->err, 0, sizeof(int), c->st));
+        CK(cudaMemsetAsync(c->tile_cnt, 0, sizeof(int) * c->n_tile_cnt, c->st));  // an aborted launch can leave counts behind
     }
-    CK(cudaMemcpy(&e, c->err, sizeof(int), cudaMemcpyDeviceToHost));
-    if (e) {
-        cudaMemset(c->err, 0, sizeof(int));
-        cudaMemset(c->tile_cnt, 0, sizeof(int) * c->n_tile_cnt);  // an aborted launch can leave counts behind
-        return set_err(DFB_ERR_TIMEOUT, "a GEMM stopped (code 0x%x: %s); results of this call are invalid", e,
-                       gemm_err_str(e));
-    }
+    if (kv8) CK(cudaMemsetAsync(c->kv8.status, 0, sizeof(int), c->st));
+    if (values) CK(cudaMemsetAsync(c->cnt + CNT_ERR, 0, sizeof(int), c->st));
+    if (gemm)
+        return set_err(DFB_ERR_TIMEOUT, "a GEMM stopped (code 0x%x: %s); results of this call are invalid", gemm,
+                       gemm_err_str(gemm));
+    if (kv8 & DFB_STAT_TIMEOUT) return set_err(DFB_ERR_TIMEOUT, "attention over the 8-bit cache stopped; results of this call are invalid");
+    if (kv8) return set_err(DFB_ERR_ARG, "8-bit cache: %s (status %d)", kv8 & DFB_STAT_NONFINITE ? "K or V not finite" : "bad rows", kv8);
+    if (values)
+        return set_err(DFB_ERR_STATE, values == 1 ? "a token id outside the vocabulary reached the embedding"
+                                                  : "a logits row has no finite maximum (non-finite logits)");
     return DFB_OK;
 }
 
@@ -1410,9 +1405,8 @@ static int forward_finish(dfb_ctx *c, int n) {
     int verr = 0;
     CK(cudaMemcpyAsync(&verr, c->cnt + CNT_ERR, sizeof(int), cudaMemcpyDeviceToHost, c->st));
     CK(cudaStreamSynchronize(c->st));
-    RET(check_values(c, verr));
     prof_collect(c, n);
-    return check_err(c);
+    return check_err(c, verr);
 }
 
 extern "C" int dfb_forward(dfb_ctx *c, const int32_t *tokens, int n, float *logits_host) {
@@ -1690,8 +1684,7 @@ extern "C" int dfb_gen_step_batch(dfb_ctx *c, int step, const int32_t *n_unmask_
     CK(cudaMemcpyAsync(h_seg.data(), c->seg_cnt, sizeof(int) * h_seg.size(), cudaMemcpyDeviceToHost, c->st));
     CK(cudaStreamSynchronize(c->st));
     prof_collect(c, h_cnt[CNT_M]);
-    RET(check_err(c));
-    RET(check_values(c, h_cnt[CNT_ERR]));
+    RET(check_err(c, h_cnt[CNT_ERR]));
     float fwd = 0, all = 0;
     cudaEventElapsedTime(&fwd, c->ev[0], c->ev[1]);
     cudaEventElapsedTime(&all, c->ev[0], c->ev[2]);
