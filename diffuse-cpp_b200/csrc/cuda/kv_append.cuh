@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T, kAppendThreads>
     constexpr int IPR = HD / 16;  // items per row
     __shared__ uint32_t red[3];
     __shared__ uint32_t written[4];
+    __shared__ int first_of[128];  // at given positions: the first row of a slot (positions out of order may repeat one)
     const int s = blockIdx.z, P = c.page, tid = threadIdx.x;
     const int groups = (c.n_kv + heads - 1) / heads;  // blocks of the K heads
     const int sec = (int)blockIdx.y < groups ? 0 : (int)blockIdx.y < 2 * groups ? 1 : 2;
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T, kAppendThreads>
         for (int i = a + 1 + tid; i < b; i += kAppendThreads)
             if (r.pos[i] <= r.pos[i - 1]) flag(DFB_STAT_POSITION);
     const long long pg = (long long)max(first, 0) / P + blockIdx.x;  // page of the sequence
-    if (pg >= c.max_pages || pg * P > last) return;
+    if (pg >= c.max_pages || pg * P > last || pg * P >= limit) return;
     const int p0 = (int)pg * P;
     int lo, hi;
     if (r.pos) {
@@ -233,15 +234,20 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T, kAppendThreads>
 
     if (tid < 4) written[tid] = 0;
     if (tid < 3) red[tid] = 0;
+    if (r.pos && tid < P) first_of[tid] = 0x7fffffff;
     __syncthreads();
-    const int row = lo + tid / IPR, i = (tid % IPR) * 8, slot = row < hi ? slot_of(row) : -1;
+    const int row = lo + tid / IPR, i = (tid % IPR) * 8;
+    int slot = row < hi ? slot_of(row) : -1;
     const T *src = src0 + row * tok + i;
     auto table = [&] { return r.rope + ((size_t)(p0 + slot) * (HD / 2) + i) * 2; };  // the item's cos and sin
     float2 cs[4], sn[4];
     RawItem<T> raw;
     if (slot >= 0) {
         raw.load(src + head0 * head_st, HD, vec);
-        if (i == 0) atomicOr(&written[slot >> 5], 1u << (slot & 31));
+        if (i == 0) {
+            atomicOr(&written[slot >> 5], 1u << (slot & 31));
+            if (r.pos) atomicMin(&first_of[slot], row);
+        }
         if (rotate) {
             const float4 *t = reinterpret_cast<const float4 *>(table());
 #pragma unroll
@@ -253,6 +259,10 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<T, kAppendThreads>
         }
     }
     __syncthreads();
+    if (r.pos) {
+        if (!(written[0] | written[1] | written[2] | written[3])) return;
+        if (slot >= 0 && first_of[slot] != row) slot = -1;
+    }
     const int kept = min(max(len - p0, 0), P);  // filled positions of the page; those written now do not survive
     bool survive = false;
     for (int t = 0; t < kept; t += 32) {

@@ -237,7 +237,9 @@ int dfb_linear_noalloc(const dfb_model *m, int role, int layer, const void *x_f1
 enum {
     DFB_STAT_PAGE = 1,      /* a page id outside [0, n_pages): its rows / keys were left out */
     DFB_STAT_POSITION = 2,  /* a position outside the page table or the rotation table, or not
-                               ascending: its row was left out; a length outside the page table */
+                               ascending: its row was left out; a length outside the page table.  Where
+                               positions do not ascend, rows around the break may be left out too; no position is
+                               stored twice */
     DFB_STAT_ROWS = 4,      /* row_off not ascending within [0, n_rows], or more rows than max_rows */
     DFB_STAT_NONFINITE = 8, /* K / V to be stored held NaN (stored as 0) or +-inf (the largest code); K rotated: either */
     DFB_STAT_TARGET = 16,   /* a target token >= n_vocab (its log probability is NaN), or a row index out of range */
@@ -286,7 +288,8 @@ typedef struct {
 /* Store rows.  The scale of a (page, KV head) becomes the smallest power of two 2^e, e >= -64,
  * with max |x| <= 448 * 2^e over the values the call writes there; while positions of that page
  * below len[s] keep their values it does not shrink, and where it grows their codes are
- * re-rounded once to the new scale.  Rows of different sequences must lie in different pages. */
+ * re-rounded once to the new scale.  The pages that a call writes must all be different ones, within a
+ * sequence and between sequences. */
 int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_t *status, void *stream);
 
 /* Attention of query rows over the cache: for each row and query head h,
