@@ -521,7 +521,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                                 for (int e = 0; e < 8; e++) reinterpret_cast<T *>(at)[e] = from[e];
                         }
-                        cp_async_arrive(&bar_raw_q[w]);
+                        // (cp.async's arrival does not wait for plain stores, nor order them)
+                        if (vec) cp_async_arrive(&bar_raw_q[w]);
+                        else mbar_arrive(&bar_raw_q[w]);
                     }
                 }
                 const int rs = n % kTcRaw, cs = n % kTcSlots, g = n >> 1;
