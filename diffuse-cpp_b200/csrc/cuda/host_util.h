@@ -13,9 +13,11 @@ int set_err(int code, const char *fmt, ...);
 #define CK(call)                                                                                   \
     do {                                                                                           \
         cudaError_t e_ = (call);                                                                   \
-        if (e_ != cudaSuccess)                                                                     \
+        if (e_ != cudaSuccess) {                                                                   \
+            cudaGetLastError(); /* else the next launch's check finds it */                        \
             return set_err(e_ == cudaErrorMemoryAllocation ? DFB_ERR_NOMEM : DFB_ERR_CUDA,         \
                            "%s failed: %s (%s:%d)", #call, cudaGetErrorString(e_), __FILE__, __LINE__); \
+        }                                                                                          \
     } while (0)
 #define RET(x)                 \
     do {                       \

@@ -57,3 +57,13 @@ def test_a_time_out_does_not_hide_behind_bad_values(pkg, model):
     assert rc == ERR_TIMEOUT, (rc, dfb.dfb_last_error())
     assert (ctx.forward(GOOD) == want).all()
     ctx.close()
+
+
+def test_a_failed_allocation_is_reported_once(pkg, model):
+    ctx = pkg.Context(model, 0)
+    want = ctx.forward(GOOD)
+    # no GPU holds the activations of so many positions: the first allocation fails
+    with pytest.raises(pkg.DiffuseError, match="memory"):
+        ctx.score(np.zeros(60_000_000, np.int32))
+    assert (ctx.forward(GOOD) == want).all()
+    ctx.close()
