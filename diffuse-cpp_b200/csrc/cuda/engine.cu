@@ -802,6 +802,7 @@ static void ctx_free_buffers(dfb_ctx *c) {
                   c->kv8.scale, c->kv8.pages, c->kv8.row_off, c->kv8.len, c->kv8.status, c->kv8.iota, c->kv8.q, c->kv8.o,
                   c->kv8.ws};
     for (void *p : ps) cudaFree(p);
+    c->gen_active = false;  // a generation's state went with them
     const bool kv8_on = c->kv8.on;
     c->kv8 = dfb_ctx::Kv8{};
     c->kv8.on = kv8_on;
@@ -1329,7 +1330,6 @@ extern "C" int dfb_ctx_set_kv8(dfb_ctx *c, int on) {
     CK(cudaStreamSynchronize(c->st));
     const int cap = c->cap;
     ctx_free_buffers(c);
-    c->gen_active = false;
     c->kv8.on = on != 0;
     return cap ? ctx_reserve(c, cap) : DFB_OK;
 }
@@ -1358,6 +1358,7 @@ extern "C" int dfb_ctx_stream(dfb_ctx *c, void **stream) {
 // Segment layout of the context's state: offsets [n_seg + 1] and finished flags (all 0).
 static int set_segments(dfb_ctx *c, const std::vector<int> &off) {
     const int n = (int)off.size() - 1;
+    c->gen_active = false;  // (a generation in progress ends here, whatever becomes of the new layout)
     CK(cudaMemcpyAsync(c->seg_off, off.data(), sizeof(int) * off.size(), cudaMemcpyHostToDevice, c->st));
     CK(cudaMemsetAsync(c->done, 0, n, c->st));
     c->n_seg = n;
@@ -1393,7 +1394,6 @@ static int forward_tokens(dfb_ctx *c, const int32_t *tokens, int n) {
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= V) return set_err(DFB_ERR_ARG, "token %d at %d outside [0, %d)", tokens[i], i, V);
     RET(ctx_reserve(c, n));
-    c->gen_active = false;
     RET(set_segments(c, {0, n}));
     CK(cudaMemcpyAsync(c->seq, tokens, n * sizeof(int32_t), cudaMemcpyHostToDevice, c->st));
     CK(cudaMemsetAsync(c->masked, 0, n, c->st));

@@ -67,3 +67,40 @@ def test_a_failed_allocation_is_reported_once(pkg, model):
         ctx.score(np.zeros(60_000_000, np.int32))
     assert (ctx.forward(GOOD) == want).all()
     ctx.close()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_generation_ends_when_its_buffers_go(pkg, model, bits):
+    """A call that replaces a context's buffers and fails, or drops them, leaves no generation that a step could
+    go on with."""
+    ctx = pkg.Context(model, 0, kv_bits=bits)
+    p = pkg.SamplerParams(n_steps=4, remasking=0, use_cache=1)
+    want = ctx.forward(GOOD)
+
+    def refused():
+        with pytest.raises(pkg.DiffuseError, match="gen_begin"):
+            ctx.gen_step(1, 2, False)
+
+    def begun():
+        ctx.gen_begin(np.zeros(0, np.int32), 8, p)
+
+    # no GPU holds the activations of so many positions: the first allocation fails
+    many = np.zeros(60_000_000, np.int32)
+    begun()
+    with pytest.raises(pkg.DiffuseError):
+        ctx.gen_begin(many, 8, p)
+    refused()
+    assert (ctx.forward(GOOD) == want).all()
+    begun()
+    with pytest.raises(pkg.DiffuseError):
+        ctx.score(many)
+    refused()
+    begun()
+    assert pkg.native()[0].dfb_ctx_set_kv8(ctx.engine, int(bits == 8)) == 0
+    refused()
+    assert (ctx.forward(GOOD) == want).all()
+    begun()
+    ctx.linear(pkg.WO, 0, np.ones((300, MINI_LLADA["n_embd"]), np.float32))  # more rows than the context had buffers for
+    refused()
+    assert (ctx.forward(GOOD) == want).all()
+    ctx.close()
