@@ -152,18 +152,19 @@ struct AttnPlan {
 // 95, 61, 75 us).
 constexpr int kShortTiles = 12;
 AttnPlan attn_plan(const dfb_kv_cache &c, const dfb_kv_attn &a, int n_sm) {
-    const int64_t packed = (int64_t)a.max_rows * (a.n_q / c.n_kv), key_tiles = (a.max_keys + kKeyTile - 1) / kKeyTile;
+    const int64_t rep = a.n_q / c.n_kv, packed = a.max_rows * rep, key_tiles = ((int64_t)a.max_keys + kKeyTile - 1) / kKeyTile;
     auto plan = [&](int rows, int64_t ctas) {
         AttnPlan p;
+        const int64_t tiles = (packed + rows - 1) / rows, base = tiles * c.n_kv * c.n_seq;
         p.rows = rows;
-        p.tiles = (int)((packed + rows - 1) / rows);
-        const int64_t base = (int64_t)p.tiles * c.n_kv * c.n_seq;
+        // launched: no sequence has more rows than there are (the splits, and with them the workspace, go by max_rows alone)
+        p.tiles = (int)std::min<int64_t>(tiles, (a.n_rows * rep + rows - 1) / rows);
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({ctas / std::max<int64_t>(base, 1), key_tiles / 4, kMaxSplits}));
         return p;
     };
     if (packed <= 64) return plan(packed <= 16 ? 16 : packed <= 32 ? 32 : 64, 2 * n_sm);
     const AttnPlan p = plan(64, n_sm);
-    const bool alone = (int64_t)p.tiles * c.n_kv * c.n_seq <= n_sm;
+    const bool alone = (packed + 63) / 64 * c.n_kv * c.n_seq <= n_sm;
     return alone && key_tiles <= (int64_t)kShortTiles * p.splits ? p : plan(kTcRows, n_sm);
 }
 size_t attn_ws_bytes(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p) {
@@ -225,7 +226,7 @@ int attn_t(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, float
         default: RET((attn_tc_launch<T, HD>(c, a, p, parts, tk, tv, vec, dev, n_sm, status, st)));
     }
     if (p.splits > 1) {
-        const int64_t per_seq = (int64_t)a.max_rows * a.n_q;
+        const int64_t per_seq = (int64_t)std::min(a.max_rows, a.n_rows) * a.n_q;
         CK(launch_k(kv_attn_join_kernel<T, HD>, dim3((unsigned)((per_seq + 3) / 4), c.n_seq), dim3(128), 0, st, true, c, a, parts));
     }
     return DFB_OK;
@@ -266,7 +267,8 @@ extern "C" int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_
     bool vec = vec_ok(r->k, r->type, r->k_tok, r->k_head) && vec_ok(r->v, r->type, r->v_tok, r->v_head);
     if (r->q) vec = vec && vec_ok(r->q, r->type, r->q_tok, r->q_head) && vec_ok(r->q_out, r->type, r->q_out_tok, r->q_out_head);
     // pages a sequence's rows can touch: consecutive positions n / page + 2 at most, given positions any of them
-    const int64_t most = r->pos ? c->max_pages : std::min<int64_t>(c->max_pages, ((int64_t)r->max_rows + c->page - 2) / c->page + 1);
+    const int64_t rows = std::min(r->max_rows, r->n_rows);
+    const int64_t most = r->pos ? c->max_pages : std::min<int64_t>(c->max_pages, (rows + c->page - 2) / c->page + 1);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     auto go = [&](auto t) {
         using T = decltype(t);
