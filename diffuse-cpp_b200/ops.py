@@ -76,6 +76,13 @@ def _empty(like, shape, dtype, index, stream):
         return like.new_empty(shape, dtype=dtype)
 
 
+def _fits(sizes):
+    """Sizes (all of them or-ed together) go to the library as int32: a larger one would arrive as another
+    number.  (Negative ones are for the library to refuse.)"""
+    if sizes >> 31 not in (0, -1):
+        raise ValueError("a size does not fit 32 bits")
+
+
 # (device indices are compared as integers: a call's checks take a few microseconds, and its kernel may not
 # take more)
 def _ints(name, t, index, n=None):
@@ -131,6 +138,7 @@ class PagedKV:
     def set_pages(self, pages):
         if pages.dim() != 2:
             raise ValueError("pages is [n_seq, max_pages]")
+        _fits(pages.shape[0] | pages.shape[1] | self.n_pages | self.n_kv)
         ptr = _ints("pages", pages, self._index)
         self.pages, self._n_seq = pages, pages.shape[0]
         self._ws = {}  # workspace sizes by the sizes of a call
@@ -152,6 +160,7 @@ def kv_append(cache: PagedKV, k, v, row_off, lens, *, max_rows: int, pos=None, r
     if k.dim() != 3 or typ is None:
         raise ValueError("k is [n_rows, n_kv, head_dim] in f32, f16 or bf16")
     n = k.shape[0]
+    _fits(n | max_rows)
     sk = _rows("k", k, k.dtype, d, (n, cache.n_kv, hd))
     sv = _rows("v", v, k.dtype, d, (n, cache.n_kv, hd))
     r = _KvRows(k.data_ptr(), v.data_ptr(), typ, n, max_rows, sk[0], sk[1], sv[0], sv[1], _ints("row_off", row_off, d, cache._n_seq + 1),
@@ -159,6 +168,7 @@ def kv_append(cache: PagedKV, k, v, row_off, lens, *, max_rows: int, pos=None, r
     if rope is not None:
         if rope.dtype is not torch.float32 or not rope.is_contiguous() or rope.get_device() != d or rope.shape[1:] != (hd // 2, 2):
             raise ValueError(f"rope must be a contiguous float32 tensor [n_positions, {hd // 2}, 2] on {cache.device}")
+        _fits(rope.shape[0])
         r.rope, r.n_rope = rope.data_ptr(), rope.shape[0]
     if (q is None) != (q_out is None):
         raise ValueError("q and q_out go together")
@@ -166,6 +176,7 @@ def kv_append(cache: PagedKV, k, v, row_off, lens, *, max_rows: int, pos=None, r
         if q.dim() != 3:
             raise ValueError("q is [n_rows, n_q, head_dim]")
         n_q = q.shape[1]
+        _fits(n_q)
         sq = _rows("q", q, k.dtype, d, (n, n_q, hd))
         so = _rows("q_out", q_out, k.dtype, d, (n, n_q, hd))
         r.n_q, r.q, r.q_out = n_q, q.data_ptr(), q_out.data_ptr()
@@ -185,6 +196,7 @@ def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: i
     if q.dim() != 3 or typ is None or typ == F32:
         raise ValueError("q is [n_rows, n_q, head_dim] in f16 or bf16")
     n, n_q, hd = q.shape
+    _fits(n | n_q | max_rows | max_keys)
     sq = _rows("q", q, q.dtype, d, (n, n_q, cache.head_dim))
     if out is None:
         out = _empty(q, (n, n_q, hd), q.dtype, d, stream)
@@ -212,6 +224,7 @@ def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: i
 
 def kv_attention_workspace(cache: PagedKV, *, n_q: int, n_rows: int, max_rows: int, max_keys: int) -> int:
     """Bytes of workspace a kv_attention call of these sizes needs (0: none)."""
+    _fits(n_q | n_rows | max_rows | max_keys)
     a = _KvAttn(type=F16, n_q=n_q, n_rows=n_rows, max_rows=max_rows, max_keys=max_keys, scale=1.0)
     need = C.c_size_t()
     _ck(_fn("dfb_kv_attention_workspace")(cache._ref, C.addressof(a), C.addressof(need)))
@@ -229,6 +242,7 @@ def token_logprobs(logits, targets=None, *, top_k: int = 0, rows=None, status=No
         raise ValueError("logits: the last dimension must be contiguous")
     d, v = logits.get_device(), logits.shape[1]
     n = logits.shape[0] if rows is None else rows.numel()
+    _fits(n | v | logits.shape[0] | top_k)
     k = max(top_k, 0)
     tp = _ints("targets", targets, d, n)
     # one allocation: logprob, entropy, top_logprob, then the ids
