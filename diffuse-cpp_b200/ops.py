@@ -19,6 +19,7 @@ from . import BF16, F16, F32, DiffuseError, native
 
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _P, _I32, _I64 = C.c_void_p, C.c_int32, C.c_int64
+_MAX_WS = 64  # workspace sizes a cache remembers: a decoding loop's bound of the keys is another one at each step
 
 
 class _KvCache(C.Structure):
@@ -208,10 +209,12 @@ def kv_attention(cache: PagedKV, q, row_off, lens, *, max_rows: int, max_keys: i
                 so[0], so[1], _ints("row_off", row_off, d, cache._n_seq + 1), _ints("lens", lens, d, cache._n_seq),
                 _ints("vis", vis, d, n), None if lse is None else lse.data_ptr())
     if workspace is None:
-        need = cache._ws.get((n_q, n, max_rows, max_keys))
+        sizes = (n_q, n, max_rows, max_keys)
+        need = cache._ws.get(sizes)
         if need is None:
-            need = cache._ws[n_q, n, max_rows, max_keys] = kv_attention_workspace(cache, n_q=n_q, n_rows=n, max_rows=max_rows,
-                                                                                  max_keys=max_keys)
+            if len(cache._ws) >= _MAX_WS:
+                cache._ws.clear()
+            need = cache._ws[sizes] = kv_attention_workspace(cache, n_q=n_q, n_rows=n, max_rows=max_rows, max_keys=max_keys)
         if need:
             workspace = _empty(q, (need,), torch.uint8, d, stream)
     elif workspace.get_device() != d or not workspace.is_contiguous():

@@ -61,3 +61,17 @@ def test_sizes_that_fit_go_on(pkg, cache):
         ops.kv_append(cache, k, k, ints(2), ints(1), max_rows=2**31 - 1)
     with pytest.raises(AssertionError, match="dfb_kv_attention_workspace"):
         ops.kv_attention_workspace(cache, n_q=2, n_rows=3, max_rows=-1, max_keys=2**31 - 1)  # (the library refuses the negative one)
+
+
+def test_a_decoding_loop_leaves_nothing_behind(pkg, cache, monkeypatch):
+    """Each step's bound of the keys is another one: what a cache remembers of the calls stays small, and calls of
+    the same sizes ask the library once."""
+    ops = pkg.ops
+    asked = []
+    monkeypatch.setattr(ops, "_fn", lambda name: lambda *a: asked.append(name) or 0)
+    q = torch.zeros(1, N_KV, HD, dtype=torch.float16)
+    for keys in range(1, 3001):
+        for _layer in range(2):
+            ops.kv_attention(cache, q, ints(2), ints(1), max_rows=1, max_keys=keys)
+    assert len(cache._ws) <= 100
+    assert asked.count("dfb_kv_attention_workspace") == 3000 and asked.count("dfb_kv_attention") == 6000
