@@ -89,6 +89,25 @@ int check_rows(const char *what, const void *p, int type, int64_t tok, int64_t h
     if (tok < 0 || head < 0) return set_err(DFB_ERR_ARG, "%s has a negative stride", what);
     return DFB_OK;
 }
+// Whether rows of an output [n][heads][head_dim] share elements (a broadcast view, say): blocks would write them
+// at the same time.
+bool rows_overlap(int64_t n, int64_t tok, int64_t heads, int64_t head, int hd) {
+    if ((n > 1 && tok < hd) || (heads > 1 && head < hd)) return true;
+    if (n == 1 || heads == 1) return false;
+    const __int128 t = tok, h = head;
+    if (t >= (heads - 1) * h + hd || h >= (n - 1) * t + hd) return false;  // one dimension within the other's steps
+    for (int64_t i = 1; i < heads; i++) {  // neither: the tokens whose rows of head 0 lie next to token 0's row of head i
+        const __int128 at = i * h, k = at / t;
+        if ((k < n && at - k * t < hd) || (k + 1 < n && (k + 1) * t - at < hd)) return true;
+    }
+    return false;
+}
+int check_out(const char *what, const void *p, int type, int64_t n, int64_t tok, int64_t heads, int64_t head, int hd) {
+    RET(check_rows(what, p, type, tok, head));
+    if (rows_overlap(n, tok, heads, head, hd))
+        return set_err(DFB_ERR_ARG, "%s: rows overlap (strides of %lld and %lld elements)", what, (long long)tok, (long long)head);
+    return DFB_OK;
+}
 // Whether eight consecutive values of every row can be moved as 16-byte pieces.
 bool vec_ok(const void *p, int type, int64_t tok, int64_t head) {
     const int64_t n = 16 / type_size(type);
@@ -258,7 +277,7 @@ extern "C" int dfb_kv_append(const dfb_kv_cache *c, const dfb_kv_rows *r, int32_
     if (r->q) {
         if (r->n_q <= 0 || r->n_q > 8192) return set_err(DFB_ERR_ARG, "%d query heads", r->n_q);
         RET(check_rows("q", r->q, r->type, r->q_tok, r->q_head));
-        RET(check_rows("q_out", r->q_out, r->type, r->q_out_tok, r->q_out_head));
+        RET(check_out("q_out", r->q_out, r->type, r->n_rows, r->q_out_tok, r->n_q, r->q_out_head, c->head_dim));
     }
     DeviceGuard g;
     RET(g.enter(c->k, "the cache"));
@@ -295,7 +314,7 @@ extern "C" int dfb_kv_attention(const dfb_kv_cache *c, const dfb_kv_attn *a, voi
     RET(check_attn(c, a));
     if (a->n_rows == 0 || a->max_rows == 0) return DFB_OK;
     RET(check_rows("q", a->q, a->type, a->q_tok, a->q_head));
-    RET(check_rows("out", a->out, a->type, a->out_tok, a->out_head));
+    RET(check_out("out", a->out, a->type, a->n_rows, a->out_tok, a->n_q, a->out_head, c->head_dim));
     if (!a->row_off || !a->len) return set_err(DFB_ERR_ARG, "null row offsets or lengths");
     DeviceGuard g;
     RET(g.enter(c->k, "the cache"));

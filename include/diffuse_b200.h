@@ -247,7 +247,8 @@ enum {
     DFB_STAT_LOGITS = 32    /* a logits row with NaN or +inf (its outputs are NaN, its ids -1) */
 };
 
-/* Element types of caller tensors (GGML ids): F32 0, F16 1, BF16 30. */
+/* Element types of caller tensors (GGML ids): F32 0, F16 1, BF16 30.  Inputs may be broadcast views (strides of
+ * 0); the rows of an output must not share elements. */
 
 /* A paged K/V cache in 8 bits.  A page holds `page` consecutive positions of one sequence, for
  * every KV head: E4M3 codes [n_pages][n_kv][page][head_dim] for K and for V, and one f32 scale
