@@ -265,9 +265,11 @@ class Context:
     """diffuse_context: device buffers + stream of one generation at a time."""
 
     def __init__(self, model: Model, n_ctx: int = 0, n_threads: int = 4, kv_bits: int = 32):
-        """kv_bits 8: the K/V kept between steps in 8 bits (dfb_ctx_set_kv8; heads of 64 or 128)."""
+        """kv_bits 8: the K/V kept between steps in 8 bits (dfb_ctx_set_kv8; heads of 64 or 128, one GPU)."""
         if kv_bits not in (8, 32):
             raise ValueError("kv_bits must be 8 or 32")
+        if kv_bits == 8 and model.tp_size > 1:
+            raise DiffuseError("the 8-bit cache is not supported on a tensor-parallel model")
         self.model = model
         self._h = native()[1].dfc_context_new(model._h, n_ctx, n_threads)
         if not self._h:

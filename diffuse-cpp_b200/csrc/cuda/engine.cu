@@ -1325,6 +1325,8 @@ extern "C" int dfb_ctx_set_kv8(dfb_ctx *c, int on) {
     if (!c) return set_err(DFB_ERR_ARG, "null context");
     if (on && c->m->hd != 64 && c->m->hd != 128)
         return set_err(DFB_ERR_UNSUPPORTED, "the 8-bit cache holds heads of 64 or 128, the model's have %d", c->m->hd);
+    // (a rank whose K or V are not finite stops with an error of its own, and the others would wait for it)
+    if (on && c->m->tp_size > 1) return set_err(DFB_ERR_UNSUPPORTED, "the 8-bit cache on a tensor-parallel model");
     std::lock_guard<std::mutex> lk(device_lock(c->m->device));
     CK(cudaSetDevice(c->m->device));
     CK(cudaStreamSynchronize(c->st));

@@ -101,8 +101,8 @@ void dfb_ctx_free(dfb_ctx *c);
  * f32: a quarter of the memory and of the bytes each step's attention reads.  K and V rows are stored
  * by dfb_kv_append (pages of 64 positions of one sequence), attention is dfb_kv_attention with Q and
  * the output rounded to f16; everything else is as before.  Stored values are off by up to 1 part in
- * 16, so logits move by some percent.  Heads of 64 or 128.  A generation in progress is dropped; may
- * be called with on = 0 to go back. */
+ * 16, so logits move by some percent.  Heads of 64 or 128, not with tensor parallelism.  A generation
+ * in progress is dropped; may be called with on = 0 to go back. */
 int dfb_ctx_set_kv8(dfb_ctx *c, int on);
 
 /* diffuse_forward (diffuse-graph.cpp:676-680): full forward over n host tokens, logits
