@@ -7,6 +7,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -50,18 +51,20 @@ class DeviceGuard {
     int dev_ = -1, old_ = -1;
 };
 
-// Compute capability and SM count, looked up once per device.
+// Compute capability and SM count, looked up once per device.  (Calls of several threads may overlap: what they
+// share is atomic, and whoever finds it unset sets it to the same value.)
 int device_props(int dev, int *n_sm) {
-    static int sms[64] = {0};
+    static std::atomic<int> sms[64];
     if (dev < 0 || dev >= 64) return set_err(DFB_ERR_UNSUPPORTED, "device %d", dev);
-    if (!sms[dev]) {
-        int major = 0, n = 0;
+    int n = sms[dev];
+    if (!n) {
+        int major = 0;
         CK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
         CK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
         if (major != 10) return set_err(DFB_ERR_UNSUPPORTED, "device %d is sm_%d; this build targets sm_100a", dev, 10 * major);
         sms[dev] = n;
     }
-    *n_sm = sms[dev];
+    *n_sm = n;
     return DFB_OK;
 }
 
@@ -195,7 +198,7 @@ int attn_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &p, 
                 const CUtensorMap &tv, bool vec, int dev, int32_t *status, cudaStream_t st) {
     const auto kern = kv_attn_kernel<T, HD, MW, KW>;
     constexpr int smem = KvSmem<HD, MW, KW>::bytes;
-    static bool attr_set[64] = {false};
+    static std::atomic<bool> attr_set[64];
     if (!attr_set[dev]) {
         CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         attr_set[dev] = true;
@@ -211,7 +214,7 @@ int attn_tc_launch(const dfb_kv_cache &c, const dfb_kv_attn &a, const AttnPlan &
     const auto kern = kv_attn_tc_kernel<T, HD>;
     constexpr int smem = TcSmem<HD>::bytes;
     static_assert(smem <= 232448, "shared memory of one CTA");
-    static bool attr_set[64] = {false};
+    static std::atomic<bool> attr_set[64];
     if (!attr_set[dev]) {
         CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         attr_set[dev] = true;
