@@ -114,15 +114,31 @@ template <typename T>
 struct LpBatch {
     static constexpr int PER = 16 / sizeof(T), N = 16, NV = N / PER;
     uint4 raw[NV];
-    __device__ __forceinline__ float at(int i) const {
-        const uint4 &u = raw[i / PER];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        const int e = i % PER;
-        if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
-        const uint32_t h = w[e / 2];
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e & 1 ? h & 0xffff0000u : h << 16);
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4 &u = raw[i / 4];
+        return i % 4 == 0 ? u.x : i % 4 == 1 ? u.y : i % 4 == 2 ? u.z : u.w;
+    }
+    __device__ __forceinline__ static float half_of(uint32_t h, int e) {  // of two 16-bit values
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(e ? h & 0xffff0000u : h << 16);
         const __half2 p = *reinterpret_cast<const __half2 *>(&h);
-        return e & 1 ? __high2float(p) : __low2float(p);
+        return e ? __high2float(p) : __low2float(p);
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(word(i));
+        return half_of(word(i / 2), i % 2);
+    }
+    // Values 2 i and 2 i + 1 where i is not known to the compiler.
+    __device__ __forceinline__ float2 pair(int i) const {
+        constexpr int W = sizeof(T) / 2;  // words of a pair
+        uint32_t w[W];
+#pragma unroll
+        for (int e = 0; e < W; e++) {
+            w[e] = word(e);
+#pragma unroll
+            for (int c = 1; c < N / 2; c++) w[e] = c == i ? word(W * c + e) : w[e];
+        }
+        if constexpr (W == 2) return make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        return make_float2(half_of(w[0], 0), half_of(w[0], 1));
     }
 };
 
@@ -245,12 +261,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const dfb
         if (LpSum::wide(sum.m)) {
             const float2 nm = make_float2(-sum.m, -sum.m);
 #pragma unroll 1  // (unrolled it costs the usual rows beside it 2 %)
-            for (int e = 0; e < B::N; e += 2) {
-                float2 f = make_float2(b.at(0), b.at(1));
-#pragma unroll
-                for (int c = 2; c < B::N; c += 2) f = c == e ? make_float2(b.at(c), b.at(c + 1)) : f;
-                term(mul2(add2(f, nm), l2e));
-            }
+            for (int e = 0; e < B::N / 2; e++) term(mul2(add2(b.pair(e), nm), l2e));
         } else {
             const float nb = -LpSum::base(sum.m);
 #pragma unroll
