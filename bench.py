@@ -1,5 +1,5 @@
 #!/usr/bin/env python
-"""Benchmark of the denoising hot path (BASELINE.json metric: denoised tok/s per B200,
+"""Benchmark of the denoising hot path (denoised tok/s per B200,
 LLaDA-8B Q4_K_M, B=256, 16 steps; ms per step).
 
 One bench "step" = one diffuse_generate call of the headline configuration (config 2):
@@ -159,7 +159,7 @@ def c2_algorithmic_flops(hp, n_active_per_step, n_keys):
     return sum(m * (per_row + att) for m in n_active_per_step)
 
 
-# Architectures of BASELINE.json's configs, for the reference arm (which imports nothing
+# Architectures of LLaDA-8B and Dream-7B, for the reference arm (which imports nothing
 # from the product package); the product's copies are diffuse-cpp_b200/__init__.py's.
 ARCH = {
     "llada": dict(is_dream=0, n_vocab=126464, n_embd=4096, n_head=32, n_head_kv=32, n_layer=32, n_ff=12288,

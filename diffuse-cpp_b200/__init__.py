@@ -71,7 +71,7 @@ class SynthSpec(C.Structure):
 
 SCHEMES = {"f32": 0, "f16": 1, "q8_0": 2, "q4_k_m": 3}
 
-# Architectures of BASELINE.json's configs (LLaDA-8B, Dream-7B).
+# Architectures of LLaDA-8B and Dream-7B.
 LLADA_8B = dict(is_dream=0, n_vocab=126464, n_embd=4096, n_head=32, n_head_kv=32, n_layer=32, n_ff=12288,
                 n_ctx=4096, mask_token_id=126336, rope_theta=500000.0, rms_norm_eps=1e-5, with_bias=0)
 DREAM_7B = dict(is_dream=1, n_vocab=152064, n_embd=3584, n_head=28, n_head_kv=4, n_layer=28, n_ff=18944,

@@ -66,7 +66,7 @@ __device__ __forceinline__ float rot_odd(float x, float c, float y, float s, flo
 }
 
 // (a c - b s, a s + b c) of two pairs, each within 1.5 units in the last place: a product's rounding
-// error is taken back.  (A zero error is +0 here, so that taking it back keeps the sign of a zero.)
+// error is taken back (Kahan's difference of two products).  (A zero error is +0 here, so that taking it back keeps the sign of a zero.)
 __device__ __forceinline__ void rot_near(float2 &a, float2 &b, float2 c, float2 s) {
     const float2 minus = make_float2(-1.f, -1.f), ns = mul2(s, minus);
     const float2 p = mul2(b, ns), q = mul2(a, s);
@@ -160,12 +160,12 @@ __device__ __forceinline__ uint2 encode8(const float2 *v, float f) {
 // a value.  rot_near's four, for two values at a time, decide every code but those whose value lies within
 // kRotTol of a border of two codes (one in 10^5), and the scale unless the maximum lies that near to
 // 448 * 2^e; those are worked out again with rot_odd, from memory, so that the usual path keeps its
-// registers.  bf16, 32768 rows of 32 + 32 + 32 heads of 128, pages of 64: 321 us, 4.2 TB/s (520 us with
-// scalar arithmetic and rows loaded when they are due); f32, 4096 rows: 75 us, 4.0 TB/s.  What is left is
+// registers.  bf16, 32768 rows of 32 + 32 + 32 heads of 128, pages of 64: 322 us, 4.2 TB/s (520 us with
+// scalar arithmetic and rows loaded when they are due); f32, 4096 rows: 77 us, 3.9 TB/s.  What is left is
 // the wait for a head's rows and for its maximum (the barrier); half the issue slots are idle.  Rows
 // three heads ahead through shared memory gave 314 us, and 95 us for f32: not worth their memory.
 // 1024 threads of an SM with 64 registers each; f32 rows, twice as long, 512 with 128 where a page allows
-// (4096 rows: 75 us, with 1024 and spills 82).
+// (4096 rows: 77 us, with 1024 and spills 82).
 template <typename T, int N>
 constexpr int kAppendCtas = (sizeof(T) == 2 || N == 1024 ? 1024 : 512) / N;
 

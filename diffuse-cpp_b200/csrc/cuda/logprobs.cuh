@@ -15,9 +15,10 @@
 //
 // Bound: the row read once from memory, and issue slots beside it: four instructions and one ex2 a value,
 // one more for the batch's largest, two more where alternatives are wanted.  2048 rows of 152064 bf16:
-// 176 us, 3.5 TB/s (138 us without alternatives); 256 rows of 126464 f32: 32 us, 4.0 TB/s (27).  A row is
+// 176 us, 3.5 TB/s (138 us without alternatives); 256 rows of 126464 f32: 34 us, 3.8 TB/s (30).  A row is
 // split over the CTAs of a cluster (joined through distributed shared memory) where rows alone would leave
-// SMs without work: one row of 126464 in 8 CTAs takes 12 us, of which 5 are launch and first batch.
+// SMs without work: one row of 126464 in 8 CTAs takes 13 us (10 without alternatives).  Rows of one large
+// value alone (2048 x 152064 of -1e10) overflow the list and take 1006 us.
 #pragma once
 #include <cstdint>
 #include <type_traits>

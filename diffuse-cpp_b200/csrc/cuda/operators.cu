@@ -129,7 +129,7 @@ int append_t(const dfb_kv_cache &c, const dfb_kv_rows &r, int64_t pages, int n_s
     const int items = c.page * (HD / 16);  // of a page: one thread each
     if (items <= 256) kv_append_kernel<T, HD, 256><<<grid, 256, 0, st>>>(c, r, heads, vec, status);
     else if (items <= 512) kv_append_kernel<T, HD, 512><<<grid, 512, 0, st>>>(c, r, heads, vec, status);
-    else kv_append_kernel<T, HD, 1024><<<grid, 1024, 0, st>>>(c, r, heads, vec, status);
+    else if constexpr (HD == 128) kv_append_kernel<T, HD, 1024><<<grid, 1024, 0, st>>>(c, r, heads, vec, status);
     CK(cudaGetLastError());
     return DFB_OK;
 }
@@ -354,8 +354,10 @@ extern "C" int dfb_token_logprobs(const dfb_logprob_args *a, int32_t *status, vo
     RET(device_props(g.device(), &n_sm));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     // CTAs of a row (a cluster of up to 8): as many as still run all at once, with 8 KB of the
-    // row to each at least.  More of them would share out the memory's bandwidth better, but each has some
-    // 5 us of its own (first batch, threshold, joining): 256 rows of 126464 took 54 us with four.
+    // row to each at least.  More of them would share out the memory's bandwidth better, but each has a part of
+    // its own (first batch, threshold, joining): 256 f32 rows of 126464 take 37, 34 and 43 us with one, two and
+    // four, one row 30, 21, 15 and 13 with one, two, four and eight, 2048 bf16 rows of 152064 176 and 229 with
+    // one and two.
     const int64_t row_bytes = (int64_t)a->n_vocab * type_size(a->type);
     int n_cta = 1;
     while (n_cta < 8 && (int64_t)a->n_rows * n_cta * 2 <= kLpCtas * n_sm && row_bytes / (2 * n_cta) >= 8192) n_cta *= 2;

@@ -132,7 +132,7 @@ int dfb_linear(dfb_ctx *c, int role, int layer, const float *x_host, int M, floa
 int dfb_debug_stalled_linear(dfb_ctx *c, int role, int layer, const float *x_host, int M, float *y_host,
                              unsigned long long timeout_ns);
 
-/* ── tensor parallelism (the north-star's optional TP mode; no counterpart in the reference) ──
+/* ── tensor parallelism (optional; no counterpart in the reference) ──
  * Rank r of size holds heads [r H/size, (r+1) H/size) of Q/K/V/O (and their KV heads), FFN
  * features [r F/size, ...) of gate/up/down and vocabulary rows [v0, v0 + n_vocab_local) of the
  * lm_head.  O and down are row-parallel: an NCCL all-reduce of their outputs follows each (the
@@ -254,7 +254,10 @@ enum {
  * every KV head: E4M3 codes [n_pages][n_kv][page][head_dim] for K and for V, and one f32 scale
  * for each page and KV head (value = code * scale).  Position p of sequence s lies in page
  * pages[s * max_pages + p / page].  head_dim 64 or 128; page 16, 32, 64 or 128.  k, v are
- * 16-byte aligned.  The codes of positions behind a sequence's length are never used. */
+ * 16-byte aligned.  The codes of positions behind a sequence's length are never used.  What dfb_kv_append
+ * stores are finite codes and scales that are powers of two from 2^-64 to 2^120; a caller's own may be any
+ * positive scales in that range and finite codes (a NaN code of V makes the outputs of all rows that are
+ * worked on together NaN, a row whose vis ends before it among them). */
 typedef struct {
     void *k, *v;
     float *k_scale, *v_scale;
