@@ -13,7 +13,8 @@
 //   O += p' . code_v,   l += p' / sv   (= 2^(x - M), in f32 before the rounding)
 // so V's scale costs one addend of the exponent and 1 / sv one multiply-add per 16 keys, and p'
 // keeps f16's precision down to 2^-(14 + kPOff) of the largest weight however far apart the pages'
-// scales are.  out = O / l, lse = (M + log2 l) ln 2.  Rounding p' to f16 (2^-11 relative, averaged
+// scales are.  out = O / l, lse = (M + log2 l) ln 2, with the rounding of f32 numbers of the size of
+// |x| + |log2 sv| (scales of 2^-40: 2e-6).  Rounding p' to f16 (2^-11 relative, averaged
 // over the keys) is the only rounding to 16 bits before the output's own.
 #pragma once
 #include <cuda.h>
