@@ -27,11 +27,14 @@ def test_attention_loose_bounds(ops, n_seq, count, keys):  # noqa: F811
     c = kill_tail(make_cache(ops, n_seq, n_kv, hd, 64, -(-keys // 64), seed=3), lens)
     q = torch.randn((n_seq * count, n_q, hd), generator=gen(4), device="cuda").half()
     for max_rows, max_keys in ((count, INT_MAX), (n_seq * count, keys), (1 << 26, keys), (1 << 27, INT_MAX)):
-        torch.cuda.synchronize()
-        t = time.perf_counter()
-        ops.kv_attention(c, q, ints(off), ints(lens), max_rows=max_rows, max_keys=max_keys)
-        torch.cuda.synchronize()
-        assert time.perf_counter() - t < 0.5  # (a loop over all tiles that 2^26 rows could have takes seconds)
+        took = []
+        for _ in range(3):  # (the first may load the kernel)
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            ops.kv_attention(c, q, ints(off), ints(lens), max_rows=max_rows, max_keys=max_keys)
+            torch.cuda.synchronize()
+            took.append(time.perf_counter() - t)
+        assert min(took) < 0.5  # (a loop over all tiles that 2^26 rows could have takes seconds)
         check_attention(ops, c, q, off, lens, max_rows=max_rows, max_keys=max_keys)
 
 
